@@ -11,6 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GDDIM_LIB") or os.path.join(_HERE, "libgddim_amd.so")
 
 GD_MAX_LEVELS = 8
+GD_MAX_AXES = 4
 
 
 class GddimError(RuntimeError):
@@ -43,12 +44,36 @@ class ProfEntry(ctypes.Structure):
                 ("bytes", ctypes.c_double), ("launches", ctypes.c_longlong)]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_longlong), ("stride_n", ctypes.c_longlong), ("stride_h", ctypes.c_longlong)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("n_axes", ctypes.c_int),
+        ("section", ctypes.c_int * GD_MAX_AXES),
+        ("paired_halves", ctypes.c_int),
+        ("pos_type", ctypes.c_int),
+        ("pos", ctypes.c_void_p),
+        ("pos_stride_b", ctypes.c_longlong),
+        ("pos_stride_n", ctypes.c_longlong),
+        ("pos_stride_axis", ctypes.c_longlong),
+        ("freq", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
 _F = ctypes.c_float
 _D = ctypes.c_double
 _SZ = ctypes.c_size_t
+_H = ctypes.POINTER(Heads)
+_RD = ctypes.POINTER(RotaryDesc)
 
 # name -> (restype, argtypes); every symbol include/gddim_amd.h declares
 SIGNATURES = {
@@ -105,6 +130,10 @@ SIGNATURES = {
     "gd_attention": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "gd_attention_fused": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "gd_attention_block_fused": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _I, _I, _I, _P]),
+    "gd_rotary": (_I, [_RD, _H, _H, _I, _I, _P]),
+    "gd_qk_norm_rotary": (_I, [_RD, _H, _H, _H, _H, _I, _I, _P, _P, _I, _F, _P]),
+    "gd_qk_norm_rotary_backward_workspace": (_LL, [_I]),
+    "gd_qk_norm_rotary_backward": (_I, [_RD, _H, _H, _H, _H, _H, _H, _I, _I, _P, _P, _I, _F, _P, _P, _P, _P]),
 }
 
 _lib = None

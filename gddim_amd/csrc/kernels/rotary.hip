@@ -1,0 +1,363 @@
+// Rotary positions with several axes, and RMS norms of queries and keys for each head with that rotation in the same pass.
+//
+//   rotation      pair p of a head (p < R/2) belongs to axis a(p) and turns by phi = pos[token][a(p)] * freq[p]:
+//                     (a, b) -> (a cos phi - b sin phi, a sin phi + b cos phi);  channels >= R pass through
+//   norm          y = rotation(w (.) x * rho),  rho = (mean_D x^2 + eps)^-1/2
+//   its gradient  g = rotation^-1(dy);  dx = rho (g w - xh mean_D(g w xh)),  xh = x rho;  dw = sum over tokens and heads of g xh
+//
+// All three are bound by HBM: each element is read once and written once (the gradient: two reads, one write), everything between stays in
+// registers.  What would cost more than the bytes is the angle: far positions times a frequency need 64 bits before the whole turns are
+// taken off.  One wave therefore takes a token -- or, with few tokens, a share of a token's heads -- computes the R/2 cosines and sines ONCE
+// (lane p pair p) into a table of its own in LDS, and walks the token's query and key heads with them.
+//
+// Layout: a lane holds W pairs = two vectors of W channels.  (i, i + R/2) pairs: vector 0 from the first half, vector 1 from the second;
+// (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head, so norm weights
+// and the weight-gradient sums stay in registers.  LP lanes (a power of two) hold a head: the norm's sums are log2 LP shuffles, 64 / LP heads
+// are in flight per wave.  Channels that pass through are pairs with phi = 0.
+//
+// W is 16 bytes of a type where pairs, strides and addresses allow it, 8 bytes else, one pair where nothing is aligned.
+#include "../common.h"
+#include "../token_ops.h"
+
+namespace gd {
+
+namespace {
+
+template <typename T, int W> struct vec_of { typedef T type __attribute__((ext_vector_type(W))); };
+template <typename T> struct vec_of<T, 1> { typedef T type; };
+template <typename T, int W> using vec = typename vec_of<T, W>::type;
+
+template <typename T, int W> __device__ __forceinline__ void to_f32(const vec<T, W> &v, float *f) {
+    if constexpr (W == 1) f[0] = (float)v;
+    else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) f[i] = (float)v[i];
+    }
+}
+
+template <typename T, int W> __device__ __forceinline__ vec<T, W> from_f32(const float *f) {
+    if constexpr (W == 1) return (T)f[0];
+    else {
+        vec<float, W> t;
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = f[i];
+        return __builtin_convertvector(t, vec<T, W>);
+    }
+}
+
+// sine and cosine of phi = pos * freq.  phi in quarter turns and the nearest whole number of them in 64 bits; what is left, |r| <= 1/2, fits 32
+// bits.  Taylor sums on [-pi/4, pi/4]: first dropped terms x^11/11! = 1.8e-9 and x^12/12! = 1.1e-10, under half a step of a float near 1.
+__device__ __forceinline__ float2 cos_sin(double pos, double freq) {
+    const double t = pos * (freq * 0.63661977236758134308);  // 2 / pi
+    const double k = rint(t);
+    const float x = (float)((t - k) * 1.57079632679489661923);
+    const int quarter = (int)((long long)k & 3);
+    const float x2 = x * x;
+    const float s = x + x * x2 * (-1.f / 6 + x2 * (1.f / 120 + x2 * (-1.f / 5040 + x2 * (1.f / 362880))));
+    const float c = 1.f + x2 * (-0.5f + x2 * (1.f / 24 + x2 * (-1.f / 720 + x2 * (1.f / 40320 + x2 * (-1.f / 3628800)))));
+    const float cc = (quarter & 1) ? s : c, ss = (quarter & 1) ? c : s;
+    return make_float2((quarter == 1 || quarter == 2) ? -cc : cc, (quarter >= 2) ? -ss : ss);
+}
+
+__device__ __forceinline__ double load_pos(const RotaryParams &p, int b, int n, int a) {
+    const long long o = b * p.pos_sb + n * p.pos_sn + a * p.pos_sa;
+    if (p.pos_type == GD_POS_I32) return (double)static_cast<const int *>(p.pos)[o];
+    if (p.pos_type == GD_POS_I64) return (double)static_cast<const long long *>(p.pos)[o];
+    return (double)static_cast<const float *>(p.pos)[o];
+}
+
+// NC: chunks of W pairs per lane (1 unless one head needs more than 64 lanes)
+template <typename T, int W, int NC, bool HALVES, int MODE>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const int lp_log2) {
+    constexpr bool NORM = MODE != ROT_PLAIN, BWD = MODE == ROT_NORM_BWD;
+    extern __shared__ __attribute__((aligned(16))) float2 table_all[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
+    const int LP = 1 << lp_log2;
+    const int pairs = (p.D + 1) / 2, R2 = p.R / 2;
+    const int chunks = (pairs + W - 1) / W;  // W > 1: whole (the launcher's rule)
+    float2 *table = table_all + wave * (chunks * W);
+    const int sub = lane >> lp_log2;
+    const int row_step = 64 >> lp_log2;
+
+    // this lane's channels: e0[c] .. + W - 1 and e1[c] .. + W - 1
+    int e0[NC], e1[NC], ch[NC];
+    bool on0[NC], on1[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        ch[c] = (lane & (LP - 1)) + 64 * c;
+        const int pr = ch[c] * W;
+        if (!HALVES) { e0[c] = 2 * pr; e1[c] = 2 * pr + W; }
+        else if (pr < R2) { e0[c] = pr; e1[c] = R2 + pr; }
+        else { e0[c] = p.R + (pr - R2); e1[c] = p.R + (p.D - p.R + 1) / 2 + (pr - R2); }
+        on0[c] = ch[c] < chunks;
+        on1[c] = on0[c] && e1[c] < p.D;  // an odd head has one channel without a partner (W == 1)
+    }
+    float w[2][NC][2 * W], dw[2][NC][2 * W];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2 * W; ++i) {
+                    const int e = i < W ? e0[c] + i : e1[c] + i - W;
+                    const bool on = (i < W ? on0[c] : on1[c]) && p.heads[s];
+                    w[s][c][i] = 1.f;
+                    if (on && p.w[s]) w[s][c][i] = p.w_f32 ? static_cast<const float *>(p.w[s])[e] : (float)static_cast<const T *>(p.w[s])[e];
+                    dw[s][c][i] = 0.f;
+                }
+    }
+    const float inv_d = 1.f / (float)p.D;
+    const int rows = p.heads[0] + p.heads[1];
+
+    for (unsigned item = blockIdx.x * waves + wave; item < p.items; item += gridDim.x * waves) {
+        const int token = (int)(item / (unsigned)p.items_per_token);
+        const int share = (int)item - token * p.items_per_token;
+        const int b = token / p.tokens, n = token - b * p.tokens;
+        const int r_end = min(rows, (share + 1) * p.rows_per_item);
+
+        vec<T, W> v0[NC], v1[NC], g0[NC], g1[NC];
+        auto offset = [&](const HeadsView *hv, int r) __attribute__((always_inline)) {
+            const int seg = r >= p.heads[0];
+            const HeadsView &h = hv[seg];
+            return static_cast<T *>(h.p) + (b * h.sb + n * h.sn + (r - (seg ? p.heads[0] : 0)) * h.sh);
+        };
+        auto load = [&](int r) __attribute__((always_inline)) {
+            const T *src = offset(p.x, r);
+            const T *gsrc = BWD ? offset(p.dy, r) : nullptr;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                v0[c] = vec<T, W>{}; v1[c] = vec<T, W>{};
+                if (on0[c]) v0[c] = *reinterpret_cast<const vec<T, W> *>(src + e0[c]);
+                if (on1[c]) v1[c] = *reinterpret_cast<const vec<T, W> *>(src + e1[c]);
+                if constexpr (BWD) {
+                    g0[c] = vec<T, W>{}; g1[c] = vec<T, W>{};
+                    if (on0[c]) g0[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e0[c]);
+                    if (on1[c]) g1[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e1[c]);
+                }
+            }
+        };
+        int r = share * p.rows_per_item + sub;
+        if (r < r_end) load(r);  // in flight while the angles are computed
+
+        for (int pr = lane; pr < chunks * W; pr += 64) {
+            float2 cs = make_float2(1.f, 0.f);
+            if (pr < R2) {
+                int a = 0;
+#pragma unroll
+                for (int i = 0; i < ROT_MAX_AXES - 1; ++i) a += (i + 1 < p.n_axes && pr >= p.axis_end[i]);
+                cs = cos_sin(load_pos(p, b, n, a), p.freq[pr]);
+                cs.y *= p.sign;
+            }
+            table[pr] = cs;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float cs[NC][W], sn[NC][W];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float2 t = table[on0[c] ? ch[c] * W + i : 0];
+                cs[c][i] = t.x; sn[c][i] = t.y;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();  // the table is read before the next item overwrites it
+
+        // all lanes of the wave walk the same number of steps: the shuffles below need every lane of a head
+        const int steps = (r_end - share * p.rows_per_item + row_step - 1) >> (6 - lp_log2);
+        for (int it = 0; it < steps; ++it, r += row_step) {
+            const bool row_on = r < r_end;
+            float a[NC][2 * W], g[NC][2 * W];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                to_f32<T, W>(v0[c], a[c]); to_f32<T, W>(v1[c], a[c] + W);
+                if constexpr (BWD) { to_f32<T, W>(g0[c], g[c]); to_f32<T, W>(g1[c], g[c] + W); }
+            }
+            if (it + 1 < steps && r + row_step < r_end) load(r + row_step);
+            const int seg = r >= p.heads[0];
+
+            // index of a pair's two channels among the lane's 2W
+            auto turn = [&](float *y, int c) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int ia = HALVES ? i : 2 * i, ib = HALVES ? W + i : 2 * i + 1;
+                    const float u = y[ia], v = y[ib];
+                    y[ia] = u * cs[c][i] - v * sn[c][i];
+                    y[ib] = u * sn[c][i] + v * cs[c][i];
+                }
+            };
+            if constexpr (NORM) {
+                float ss = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 2 * W; ++i) ss += a[c][i] * a[c][i];
+                float gx = 0.f;
+                if constexpr (BWD) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        turn(g[c], c);
+#pragma unroll
+                        for (int i = 0; i < 2 * W; ++i) gx += g[c][i] * (seg ? w[1][c][i] : w[0][c][i]) * a[c][i];
+                    }
+                }
+                for (int m = 1; m < LP; m <<= 1) {
+                    ss += __shfl_xor(ss, m);
+                    if constexpr (BWD) gx += __shfl_xor(gx, m);
+                }
+                const float rho = 1.f / sqrtf(ss * inv_d + p.eps);
+                const float k = gx * inv_d * rho * rho;  // mean(g w xh) rho^-1 ... times xh = x rho below
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 2 * W; ++i) {
+                        const float wi = seg ? w[1][c][i] : w[0][c][i];
+                        if constexpr (BWD) {
+                            const float gi = row_on ? g[c][i] * (a[c][i] * rho) : 0.f;
+                            dw[0][c][i] += seg ? 0.f : gi;
+                            dw[1][c][i] += seg ? gi : 0.f;
+                            a[c][i] = rho * (g[c][i] * wi - a[c][i] * k);
+                        } else a[c][i] = a[c][i] * rho * wi;
+                    }
+            }
+            if (row_on) {
+                T *dst = offset(p.out, r);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    if constexpr (!BWD) turn(a[c], c);
+                    if (on0[c]) *reinterpret_cast<vec<T, W> *>(dst + e0[c]) = from_f32<T, W>(a[c]);
+                    if (on1[c]) *reinterpret_cast<vec<T, W> *>(dst + e1[c]) = from_f32<T, W>(a[c] + W);
+                }
+            }
+        }
+    }
+
+    if constexpr (BWD) {
+        // weight gradients: the wave's heads by shuffles, the workgroup's waves through LDS in wave order, one row of partials per
+        // workgroup (summed in order by rotary_dw_kernel: the same bits every time)
+        float *red = reinterpret_cast<float *>(table_all);  // [waves][2][D]
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2 * W; ++i) {
+                    float t = dw[s][c][i];
+                    for (int m = LP; m < 64; m <<= 1) t += __shfl_xor(t, m);
+                    const int e = i < W ? e0[c] + i : e1[c] + i - W;
+                    if (sub == 0 && (i < W ? on0[c] : on1[c])) red[(wave * 2 + s) * p.D + e] = t;
+                }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
+            float t = 0.f;
+            for (int k = 0; k < waves; ++k) t += red[k * 2 * p.D + i];
+            p.dw_part[(size_t)blockIdx.x * 2 * p.D + i] = t;
+        }
+    }
+}
+
+// dw[i] = sum over workgroups of their partial rows: 16 columns x 64 row groups per workgroup, added in a fixed order
+template <typename T>
+__global__ __launch_bounds__(1024) void rotary_dw_kernel(const float *part, int blocks, int D, void *dw0, void *dw1, int w_f32) {
+    __shared__ float red[64][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), grp = threadIdx.x >> 4;
+    float t = 0.f;
+    if (col < 2 * D)
+        for (int k = grp; k < blocks; k += 64) t += part[(size_t)k * 2 * D + col];
+    red[grp][threadIdx.x & 15] = t;
+    __syncthreads();
+    if (grp == 0 && col < 2 * D) {
+        double sum = 0.0;
+        for (int k = 0; k < 64; ++k) sum += (double)red[k][threadIdx.x];
+        void *dst = col < D ? dw0 : dw1;
+        const int e = col < D ? col : col - D;
+        if (!dst) return;
+        if (w_f32) static_cast<float *>(dst)[e] = (float)sum;
+        else static_cast<T *>(dst)[e] = (T)(float)sum;
+    }
+}
+
+template <typename T, int W, int NC, bool HALVES>
+int launch_mode(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks, void *dw0, void *dw1, hipStream_t s) {
+    const int chunks = ((p.D + 1) / 2 + W - 1) / W;
+    size_t lds = (size_t)4 * chunks * W * sizeof(float2);
+    switch (mode) {
+        case ROT_PLAIN: rotary_kernel<T, W, NC, HALVES, ROT_PLAIN><<<blocks, 256, lds, s>>>(p, lp_log2); break;
+        case ROT_NORM: rotary_kernel<T, W, NC, HALVES, ROT_NORM><<<blocks, 256, lds, s>>>(p, lp_log2); break;
+        case ROT_NORM_BWD:
+            if (lds < (size_t)4 * 2 * p.D * sizeof(float)) lds = (size_t)4 * 2 * p.D * sizeof(float);
+            rotary_kernel<T, W, NC, HALVES, ROT_NORM_BWD><<<blocks, 256, lds, s>>>(p, lp_log2);
+            GD_HIP(hipGetLastError());
+            rotary_dw_kernel<T><<<(2 * p.D + 15) / 16, 1024, 0, s>>>(p.dw_part, blocks, p.D, dw0, dw1, p.w_f32);
+            break;
+    }
+    GD_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int W, int NC>
+int launch_pairs(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks, void *dw0, void *dw1, hipStream_t s) {
+    return p.halves ? launch_mode<T, W, NC, true>(p, mode, lp_log2, blocks, dw0, dw1, s)
+                    : launch_mode<T, W, NC, false>(p, mode, lp_log2, blocks, dw0, dw1, s);
+}
+
+// vectors of W channels: every address a multiple of their size, pairs and pass-through channels whole vectors
+bool vec_ok(const RotaryParams &p, int W, int elem, bool bwd) {
+    const size_t bytes = (size_t)W * elem;
+    if (p.D % (2 * W) || p.R % (2 * W)) return false;
+    auto ok = [&](const HeadsView &h) {
+        return (size_t)h.p % bytes == 0 && h.sb % W == 0 && h.sn % W == 0 && h.sh % W == 0;
+    };
+    for (int s = 0; s < 2; ++s)
+        if (p.heads[s] && !(ok(p.x[s]) && ok(p.out[s]) && (!bwd || ok(p.dy[s])))) return false;
+    return true;
+}
+
+template <typename T>
+int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStream_t s) {
+    constexpr int WV = 16 / sizeof(T);
+    const bool bwd = mode == ROT_NORM_BWD;
+    const int W = vec_ok(p, WV, sizeof(T), bwd) ? WV : vec_ok(p, WV / 2, sizeof(T), bwd) ? WV / 2 : 1;
+    const int chunks = ((p.D + 1) / 2 + W - 1) / W;
+    int lp_log2 = 0;
+    while (lp_log2 < 6 && (1 << lp_log2) < chunks) ++lp_log2;
+    const int rows = p.heads[0] + p.heads[1], row_step = 64 >> lp_log2;
+    const long long tokens = (long long)p.batch * p.tokens;
+    if (tokens == 0) {
+        if (bwd) rotary_dw_kernel<T><<<(2 * p.D + 15) / 16, 1024, 0, s>>>(p.dw_part, 0, p.D, dw0, dw1, p.w_f32);
+        GD_HIP(hipGetLastError());
+        return 0;
+    }
+    // a wave takes whole tokens once they fill the chip (16 waves per CU), else a share of a token's heads, at least one step of them
+    const int max_blocks = bwd ? ROT_BWD_BLOCKS : device_cus() * 16;
+    const long long want = (long long)device_cus() * 16;
+    long long shares = tokens >= want ? 1 : (want + tokens - 1) / tokens;
+    const int steps = (rows + row_step - 1) / row_step;
+    if (shares > steps) shares = steps;
+    p.rows_per_item = (int)((steps + shares - 1) / shares) * row_step;
+    p.items_per_token = (rows + p.rows_per_item - 1) / p.rows_per_item;
+    p.items = (unsigned)(tokens * p.items_per_token);  // < 2^31: shares are taken only where tokens are few
+    unsigned blocks = (p.items + 3) / 4;
+    if (blocks > (unsigned)max_blocks) blocks = max_blocks;
+    if (W == WV && chunks <= 64) return launch_pairs<T, WV, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
+    if (W == WV / 2 && W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
+    if (chunks <= 64) return launch_pairs<T, 1, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
+    return launch_pairs<T, 1, 4>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
+}
+
+}  // namespace
+
+int launch_rotary(RotaryParams p, int dtype, RotaryMode mode, void *dw0, void *dw1, hipStream_t s) {
+    switch (dtype) {
+        case GD_F32: return launch_type<float>(p, mode, dw0, dw1, s);
+        case GD_BF16: return launch_type<__bf16>(p, mode, dw0, dw1, s);
+        case GD_F16: return launch_type<_Float16>(p, mode, dw0, dw1, s);
+    }
+    GD_CHECK(false, "unknown element type %d", dtype);
+}
+
+}  // namespace gd

@@ -1,0 +1,222 @@
+"""Token operators of the C ABI on torch device tensors: positions with several axes, norms of queries and keys with the rotation in the same
+pass, the gated feed-forward block (include/gddim_amd.h, "token operators").
+
+Tensors are float32, bfloat16 or float16 and stay in their type; work is queued on the current stream of the tensors' device, nothing
+synchronises, and every call can be captured into a graph.  The operators record no autograd graph: gradients come from the *_backward calls, and a
+tensor that requires grad is refused while grad mode is on.  No reference counterpart."""
+import ctypes
+import math
+
+from . import _abi
+from ._abi import GddimError, Heads, RotaryDesc, check
+
+_TORCH = None
+
+
+def _torch():
+    """(torch, element type codes, position type codes), imported once"""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = (torch, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}, {torch.int32: 0, torch.int64: 1, torch.float32: 2})
+    return _TORCH
+
+
+def _on_gpu(t, name):
+    torch = _torch()[0]
+    if not isinstance(t, torch.Tensor):
+        raise GddimError("%s: expected a torch tensor, got %s" % (name, type(t).__name__))
+    if not t.is_cuda:
+        raise GddimError("gddim_amd operators run on the GPU only (%s is a %s tensor); there is no CPU fallback" % (name, t.device))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise GddimError("%s requires grad: the token operators record no autograd graph; call them under torch.no_grad() and take gradients "
+                         "from the *_backward calls" % name)
+
+
+def _like(t, name, ref, ref_name):
+    _on_gpu(t, name)
+    if t.dtype != ref.dtype or t.device != ref.device:
+        raise GddimError("%s is %s on %s, %s is %s on %s: types and devices must agree" % (name, t.dtype, t.device, ref_name, ref.dtype, ref.device))
+
+
+class _Device:
+    """The tensors' device made current for a native call (a no-op when it is)."""
+
+    def __init__(self, t):
+        torch = _torch()[0]
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+        self.t = t
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return ctypes.c_void_p(_torch()[0].cuda.current_stream(self.t.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+class RotaryAxes:
+    """How the channels of a head turn with positions of one to four axes (time, height, width, ...).
+
+    sections[a] channels (even) turn with axis a, in this order; channels behind the last section pass through.  Pair j of a section turns
+    by pos * theta^(-2 j / sections[a]); `frequencies` (sum(sections) / 2 radians per unit of position) replaces these.  paired:
+    'interleaved' -- channels (2 p, 2 p + 1) -- or 'halves' -- channels (p, p + sum(sections) / 2).  Keeps one float64 table on `device`."""
+
+    def __init__(self, sections, theta=10000.0, paired="interleaved", device=None, frequencies=None):
+        torch = _torch()[0]
+        self.sections = tuple(int(s) for s in sections)
+        if not 1 <= len(self.sections) <= _abi.GD_MAX_AXES:
+            raise GddimError("RotaryAxes: %d axes, 1 to %d are supported" % (len(self.sections), _abi.GD_MAX_AXES))
+        if any(s < 2 or s % 2 for s in self.sections):
+            raise GddimError("RotaryAxes: sections %r must be even and at least 2" % (self.sections,))
+        if paired not in ("interleaved", "halves"):
+            raise GddimError("RotaryAxes: paired=%r, expected 'interleaved' or 'halves'" % (paired,))
+        if not (theta > 0.0 and math.isfinite(theta)):
+            raise GddimError("RotaryAxes: theta=%r must be positive" % (theta,))
+        self.theta, self.paired = float(theta), paired
+        if frequencies is None:
+            frequencies = [self.theta ** (-2.0 * j / s) for s in self.sections for j in range(s // 2)]
+        device = torch.device("cuda") if device is None else torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.frequencies = torch.as_tensor(frequencies, dtype=torch.float64).detach().to(device).contiguous()
+        if tuple(self.frequencies.shape) != (sum(self.sections) // 2,):
+            raise GddimError("RotaryAxes: frequencies of shape %s, expected (%d,)" % (tuple(self.frequencies.shape), sum(self.sections) // 2))
+        self.device = device
+        self._section = (ctypes.c_int * _abi.GD_MAX_AXES)(*self.sections)
+
+
+def _heads(t, name):
+    """(tensor, its view): channels adjacent, (B, N, heads, D)"""
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+    s = t.stride()
+    return t, Heads(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _check_heads(t, name, like=None, like_name=None):
+    _on_gpu(t, name) if like is None else _like(t, name, like, like_name)
+    if t.dim() != 4:
+        raise GddimError("%s has shape %s, expected (B, N, heads, D)" % (name, tuple(t.shape)))
+    if t.dtype not in _torch()[1]:
+        raise GddimError("%s is %s; float32, bfloat16 and float16 are supported" % (name, t.dtype))
+
+
+def _new(t):
+    """An output like t: its order of dimensions where t is dense with adjacent channels ((B, heads, N, D) seen as (B, N, heads, D)), else contiguous."""
+    torch = _torch()[0]
+    if t.is_contiguous() or 0 in t.stride() or 0 in t.shape:
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    out = torch.empty_like(t)
+    return out if out.stride(3) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _rotary_desc(x, pos, axes):
+    torch, types, pos_types = _torch()
+    if not isinstance(axes, RotaryAxes):
+        raise GddimError("axes: expected a RotaryAxes, got %s" % type(axes).__name__)
+    B, N, _, D = x.shape
+    _on_gpu(pos, "pos")
+    if pos.dtype not in pos_types:
+        raise GddimError("pos is %s; int32, int64 and float32 positions are supported" % pos.dtype)
+    if pos.device != x.device or axes.device != x.device:
+        raise GddimError("tensors on %s, positions on %s, axes on %s: devices must agree" % (x.device, pos.device, axes.device))
+    A = len(axes.sections)
+    ps, st = tuple(pos.shape), pos.stride()
+    if ps == (N, A):
+        st = (0,) + st
+    elif ps == (1, N, A):
+        st = (0,) + st[1:]
+    elif ps != (B, N, A):
+        raise GddimError("pos has shape %s, expected (%d, %d) or (%d, %d, %d)" % (ps, N, A, B, N, A))
+    if sum(axes.sections) > D:
+        raise GddimError("sections %r of %d channels exceed the head's %d" % (axes.sections, sum(axes.sections), D))
+    if B * N >= 1 << 31:
+        raise GddimError("%d x %d tokens do not fit 31 bits" % (B, N))
+    return RotaryDesc(types[x.dtype], B, N, D, A, axes._section, axes.paired == "halves", pos_types[pos.dtype], pos.data_ptr(), st[0], st[1], st[2],
+                      axes.frequencies.data_ptr())
+
+
+def rotary(x, pos, axes, inverse=False):
+    """Rotary positions with several axes: x (B, N, heads, D) turned by pos (N, axes) or (B, N, axes) as `axes` (RotaryAxes) says.
+
+    inverse=True turns back, which is also the gradient of the forward call.  Any strides with adjacent channels; the result keeps x's
+    order of dimensions where x is dense."""
+    _check_heads(x, "x")
+    desc = _rotary_desc(x, pos, axes)
+    out = _new(x)
+    x, xv = _heads(x, "x")
+    _, ov = _heads(out, "out")
+    with _Device(x) as stream:
+        check(_abi.lib().gd_rotary(desc, xv, ov, x.shape[2], int(bool(inverse)), stream))
+    return out
+
+
+def _norm_weight(w, name, q):
+    """(pointer, is it float32 beside another type)"""
+    torch = _torch()[0]
+    if w is None:
+        return None
+    _on_gpu(w, name)
+    if tuple(w.shape) != (q.shape[3],):
+        raise GddimError("%s has shape %s, expected (%d,)" % (name, tuple(w.shape), q.shape[3]))
+    if w.device != q.device or w.dtype not in (q.dtype, torch.float32):
+        raise GddimError("%s is %s on %s; the tensors' type %s or float32, on %s, is supported" % (name, w.dtype, w.device, q.dtype, q.device))
+    return w.contiguous()
+
+
+def _check_qk(q, k, w_q, w_k, eps):
+    _check_heads(q, "q")
+    _check_heads(k, "k", q, "q")
+    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise GddimError("q %s and k %s must agree in all but their heads" % (tuple(q.shape), tuple(k.shape)))
+    if not (0.0 <= eps < math.inf):
+        raise GddimError("eps=%r must be finite and not negative" % (eps,))
+    w_q, w_k = _norm_weight(w_q, "weight_q", q), _norm_weight(w_k, "weight_k", q)
+    if w_q is not None and w_k is not None and w_q.dtype != w_k.dtype:
+        raise GddimError("weight_q is %s, weight_k %s: their types must agree" % (w_q.dtype, w_k.dtype))
+    return w_q, w_k
+
+
+def _w_f32(q, w_q, w_k):
+    w = w_q if w_q is not None else w_k
+    return int(w is not None and w.dtype != q.dtype)
+
+
+def qk_norm_rotary(q, k, weight_q, weight_k, pos, axes, eps=1e-6):
+    """RMS norms of queries and keys for each head, then the rotation, in one pass: q (B, N, heads, D) and k (B, N, key heads, D), views of a
+    packed projection among them, weights (D,) of their type or float32 (None: ones).  Returns (q', k')."""
+    w_q, w_k = _check_qk(q, k, weight_q, weight_k, eps)
+    desc = _rotary_desc(q, pos, axes)
+    qo, ko = _new(q), _new(k)
+    (q, qv), (k, kv) = _heads(q, "q"), _heads(k, "k")
+    with _Device(q) as stream:
+        check(_abi.lib().gd_qk_norm_rotary(desc, qv, kv, _heads(qo, "q")[1], _heads(ko, "k")[1], q.shape[2], k.shape[2],
+                                           w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None,
+                                           _w_f32(q, w_q, w_k), float(eps), stream))
+    return qo, ko
+
+
+def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes, eps=1e-6):
+    """Gradients of qk_norm_rotary: (dq, dk, dweight_q, dweight_k) from those of its outputs (None for a weight that is None).  The same bits
+    every time."""
+    torch = _torch()[0]
+    w_q, w_k = _check_qk(q, k, weight_q, weight_k, eps)
+    for g, name, t in ((dq_out, "dq_out", q), (dk_out, "dk_out", k)):
+        _check_heads(g, name, q, "q")
+        if g.shape != t.shape:
+            raise GddimError("%s has shape %s, expected %s" % (name, tuple(g.shape), tuple(t.shape)))
+    desc = _rotary_desc(q, pos, axes)
+    dq, dk = _new(q), _new(k)
+    dwq, dwk = (torch.empty_like(w) if w is not None else None for w in (w_q, w_k))
+    (q, qv), (k, kv), (dq_out, gqv), (dk_out, gkv) = _heads(q, "q"), _heads(k, "k"), _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
+    lib = _abi.lib()
+    ws = torch.empty(lib.gd_qk_norm_rotary_backward_workspace(q.shape[3]), dtype=torch.uint8, device=q.device)
+    with _Device(q) as stream:
+        check(lib.gd_qk_norm_rotary_backward(desc, gqv, gkv, qv, kv, _heads(dq, "dq")[1], _heads(dk, "dk")[1], q.shape[2], k.shape[2],
+                                             w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None,
+                                             _w_f32(q, w_q, w_k), float(eps), ws.data_ptr(),
+                                             dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None, stream))
+    return dq, dk, dwq, dwk

@@ -350,6 +350,47 @@ int gd_attention_fused(const float *qk_dev, const float *vT_dev, const float *bi
 int gd_attention_block_fused(const float *q_dev, const float *k_dev, const float *vT_dev, const float *bias_dev, const float *res_dev,
                              float out_scale, float *qstats_dev, float *out_dev, int batch, int N, int C, void *stream);
 
+/* ---- token operators (no engine) --------------------------------------------------------------
+ * What a score network made of attention blocks over tokens runs beside its attention.  No reference counterpart.  All pointers are device
+ * pointers; tensors are fp32, bf16 or fp16 (GD_F32 / GD_BF16 / GD_F16), sums and statistics are kept in 32 bits.  The calls allocate
+ * nothing, only queue kernels on `stream` and may be captured into a hipGraph. */
+#define GD_F32 0
+#define GD_BF16 1
+#define GD_F16 2
+#define GD_POS_I32 0
+#define GD_POS_I64 1
+#define GD_POS_F32 2
+#define GD_MAX_AXES 4
+/* one (B, N, heads, D) tensor: strides in elements, the D channels of a head adjacent; heads may be 0 in none of the calls below */
+typedef struct gd_heads {
+    void *data;
+    long long stride_b, stride_n, stride_h;
+} gd_heads;
+/* Positions with n_axes axes (time, height, width, ...) of every token: pair p of a head's first R = sum(section) channels belongs to the
+ * axis whose section holds channel 2p and turns by pos[b][n][axis] * freq[p] (freq: R/2 doubles, radians per unit of position; the angle is
+ * formed and reduced in 64 bits).  paired_halves == 0: pairs (2p, 2p + 1); != 0: pairs (p, p + R/2).  Channels >= R pass through. */
+typedef struct gd_rotary_desc {
+    int dtype, batch, tokens, head_dim;
+    int n_axes, section[GD_MAX_AXES]; /* channels of each axis, even; 2 <= R <= head_dim <= 512 */
+    int paired_halves;
+    int pos_type;                     /* GD_POS_* */
+    const void *pos;
+    long long pos_stride_b, pos_stride_n, pos_stride_axis;  /* elements; 0 = shared */
+    const double *freq;
+} gd_rotary_desc;
+/* out = rotation(x); inverse != 0: the rotation back, which is also the gradient.  x and out may not overlap. */
+int gd_rotary(const gd_rotary_desc *d, const gd_heads *x, const gd_heads *out, int heads, int inverse, void *stream);
+/* out = rotation(w (.) x / sqrt(mean_D x^2 + eps)) for the queries and the keys of every token in one pass; w_q / w_k (D) of the tensors'
+ * type, or fp32 with w_f32 != 0, or null (ones). */
+int gd_qk_norm_rotary(const gd_rotary_desc *d, const gd_heads *q, const gd_heads *k, const gd_heads *q_out, const gd_heads *k_out, int heads_q,
+                      int heads_k, const void *w_q, const void *w_k, int w_f32, float eps, void *stream);
+/* Its gradient: dq, dk of the inputs and dw_q, dw_k (types as w; null where the weight is) from the outputs' gradients.  workspace_dev holds
+ * gd_qk_norm_rotary_backward_workspace(head_dim) bytes.  The sums over tokens and heads run in a fixed order. */
+long long gd_qk_norm_rotary_backward_workspace(int head_dim);
+int gd_qk_norm_rotary_backward(const gd_rotary_desc *d, const gd_heads *dq_out, const gd_heads *dk_out, const gd_heads *q, const gd_heads *k,
+                               const gd_heads *dq, const gd_heads *dk, int heads_q, int heads_k, const void *w_q, const void *w_k, int w_f32,
+                               float eps, void *workspace_dev, void *dw_q, void *dw_k, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,88 @@
+"""CPU tests of the token operators' boundary: argument checks of the Python wrappers and of the C entry points (which refuse before anything
+is launched), and the float64 forms that the GPU tests compare with, against autograd."""
+import ctypes
+
+import pytest
+import torch
+
+import token_reference as ref
+
+
+def test_rotary_axes_checks(native_lib):
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    for kw in (dict(sections=()), dict(sections=(2,) * 5), dict(sections=(3,)), dict(sections=(0,)), dict(sections=(4,), paired="quarters"),
+               dict(sections=(4,), theta=0.0), dict(sections=(4,), theta=float("nan")), dict(sections=(4, 4), frequencies=[1.0])):
+        with pytest.raises(GddimError):
+            ops.RotaryAxes(device="cpu", **kw)
+    axes = ops.RotaryAxes((4, 6), theta=100.0, device="cpu")
+    want = [100.0 ** (-2 * j / s) for s in (4, 6) for j in range(s // 2)]
+    assert axes.frequencies.tolist() == want and axes.frequencies.dtype == torch.float64
+
+
+def test_no_cpu_fallback(native_lib):
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    axes, x, pos = ops.RotaryAxes((4,), device="cpu"), torch.zeros(1, 2, 1, 4), torch.zeros(2, 1, dtype=torch.int64)
+    for call in (lambda: ops.rotary(x, pos, axes), lambda: ops.qk_norm_rotary(x, x, None, None, pos, axes),
+                 lambda: ops.qk_norm_rotary_backward(x, x, x, x, None, None, pos, axes), lambda: ops.rotary([1.0], pos, axes)):
+        with pytest.raises(GddimError):
+            call()
+
+
+def _desc(**kw):
+    from gddim_amd._abi import RotaryDesc
+    d = dict(dtype=0, batch=1, tokens=4, head_dim=16, n_axes=2, section=(8, 8), paired_halves=0, pos_type=0, pos=64, pos_stride_b=0, pos_stride_n=2,
+             pos_stride_axis=1, freq=64)
+    d.update(kw)
+    d["section"] = (ctypes.c_int * 4)(*d["section"])
+    return RotaryDesc(**d)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=3), dict(dtype=-1), dict(pos_type=9), dict(batch=-1), dict(batch=1 << 16, tokens=1 << 15), dict(head_dim=1), dict(head_dim=513),
+    dict(n_axes=0), dict(n_axes=5), dict(section=(8, 10)), dict(section=(8, 7)), dict(section=(8, 0)), dict(section=(8, -8)), dict(section=(2 ** 31 - 2, 8)),
+    dict(pos=None), dict(freq=None)], ids=str)
+def test_c_entry_points_refuse_descriptions(native_lib, bad):
+    """None of these reaches a launch: the fake addresses are never read."""
+    from gddim_amd._abi import Heads
+    h = Heads(64, 64, 16, 16)
+    assert native_lib.gd_rotary(_desc(**bad), h, h, 1, 0, None) != 0
+    assert native_lib.gd_last_error()
+    assert native_lib.gd_qk_norm_rotary(_desc(**bad), h, h, h, h, 1, 1, None, None, 0, 1e-6, None) != 0
+    assert native_lib.gd_qk_norm_rotary_backward(_desc(**bad), h, h, h, h, h, h, 1, 1, None, None, 0, 1e-6, 64, None, None, None) != 0
+
+
+def test_c_entry_points_refuse_arguments(native_lib):
+    from gddim_amd._abi import Heads
+    h, null, d = Heads(64, 64, 16, 16), Heads(None, 64, 16, 16), _desc()
+    assert native_lib.gd_rotary(None, h, h, 1, 0, None) != 0
+    assert native_lib.gd_rotary(d, h, null, 1, 0, None) != 0
+    assert native_lib.gd_rotary(d, None, h, 1, 0, None) != 0
+    for heads in (0, -1, 1 << 16):
+        assert native_lib.gd_rotary(d, h, h, heads, 0, None) != 0
+        assert native_lib.gd_qk_norm_rotary(d, h, h, h, h, 1, heads, None, None, 0, 1e-6, None) != 0
+    for eps in (-1.0, float("nan")):
+        assert native_lib.gd_qk_norm_rotary(d, h, h, h, h, 1, 1, None, None, 0, eps, None) != 0
+    assert native_lib.gd_qk_norm_rotary_backward(d, h, h, h, h, h, h, 1, 1, None, None, 0, 1e-6, None, None, None, None) != 0
+    assert native_lib.gd_qk_norm_rotary_backward_workspace(128) > 0
+
+
+@pytest.mark.parametrize("paired", ["interleaved", "halves"])
+def test_float64_forms_against_autograd(paired):
+    """The formulas that the GPU tests hold the kernels to, against differentiation of the forward form."""
+    g = torch.Generator().manual_seed(0)
+    x, dy = torch.randn(2, 3, 2, 14, generator=g, dtype=torch.float64), torch.randn(2, 3, 2, 14, generator=g, dtype=torch.float64)
+    w = torch.randn(14, generator=g, dtype=torch.float64)
+    phi = ref.angles(torch.randint(0, 50, (3, 2), generator=g), (4, 8), 100.0, 2, 3)
+    xa, wa = x.clone().requires_grad_(), w.clone().requires_grad_()
+    rho = 1.0 / torch.sqrt((xa * xa).mean(-1, keepdim=True) + 1e-3)
+    ia, ib = ref.pair_index((4, 8), paired)
+    y = xa * rho * wa
+    z = torch.complex(y[..., ia], y[..., ib]) * torch.polar(torch.ones_like(phi), phi)[:, :, None]
+    loss = (z.real * dy[..., ia] + z.imag * dy[..., ib]).sum() + (y[..., 12:] * dy[..., 12:]).sum()
+    dx, dw = torch.autograd.grad(loss, (xa, wa))
+    got = ref.norm_rotary_backward(dy, x, w, phi, (4, 8), paired, 1e-3)
+    assert (got[0] - dx).abs().max() < 1e-12 and (got[2] - dw).abs().max() < 1e-12
+    out = ref.norm_rotary(x, w, phi, (4, 8), paired, 1e-3)[0]
+    assert (out[..., ia] - z.real).abs().max() < 1e-12 and (out[..., ib] - z.imag).abs().max() < 1e-12
