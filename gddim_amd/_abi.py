@@ -66,6 +66,20 @@ class RotaryDesc(ctypes.Structure):
     ]
 
 
+class FfnDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("act", ctypes.c_int),
+        ("rows", ctypes.c_int),
+        ("in_", ctypes.c_int),
+        ("hidden", ctypes.c_int),
+        ("out", ctypes.c_int),
+        ("ld_x", ctypes.c_longlong),
+        ("ld_w_in", ctypes.c_longlong),
+        ("ld_w_down", ctypes.c_longlong),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
@@ -74,6 +88,7 @@ _D = ctypes.c_double
 _SZ = ctypes.c_size_t
 _H = ctypes.POINTER(Heads)
 _RD = ctypes.POINTER(RotaryDesc)
+_FD = ctypes.POINTER(FfnDesc)
 
 # name -> (restype, argtypes); every symbol include/gddim_amd.h declares
 SIGNATURES = {
@@ -134,6 +149,9 @@ SIGNATURES = {
     "gd_qk_norm_rotary": (_I, [_RD, _H, _H, _H, _H, _I, _I, _P, _P, _I, _F, _P]),
     "gd_qk_norm_rotary_backward_workspace": (_LL, [_I]),
     "gd_qk_norm_rotary_backward": (_I, [_RD, _H, _H, _H, _H, _H, _H, _I, _I, _P, _P, _I, _F, _P, _P, _P, _P]),
+    "gd_gated_ffn_workspace": (_LL, [_FD, _I]),
+    "gd_gated_ffn": (_I, [_FD, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "gd_gated_ffn_backward": (_I, [_FD, _P, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib = None

@@ -11,13 +11,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgddim_amd.so")
-SOURCES = ["engine.cpp", "plan.cpp", "options.cpp", "host_math.cpp", "kernels/igemm.hip", "kernels/igemm_bf16x3.hip", "kernels/conv3x3_halo_bf16x3.hip", "kernels/conv3x3_wino2d_f32.hip", "kernels/conv3x3_wino42_f32.hip", "kernels/conv3x3_wino2d_split6.hip", "kernels/attn_fused_f32.hip", "kernels/norm_act.hip", "kernels/update.hip", "token_ops.cpp", "kernels/rotary.hip"]
-HEADERS = ["common.h", "token_ops.h", "plan.h", "options.h", "kernels/qstats.h", "kernels/epilogue.h", "kernels/rng.h", "kernels/act.h", "../../include/gddim_amd.h"]
+SOURCES = ["engine.cpp", "plan.cpp", "options.cpp", "host_math.cpp", "kernels/igemm.hip", "kernels/igemm_bf16x3.hip", "kernels/conv3x3_halo_bf16x3.hip", "kernels/conv3x3_wino2d_f32.hip", "kernels/conv3x3_wino42_f32.hip", "kernels/conv3x3_wino2d_split6.hip", "kernels/attn_fused_f32.hip", "kernels/norm_act.hip", "kernels/update.hip", "token_ops.cpp", "kernels/rotary.hip",
+           "kernels/gated_ffn_bf16.hip", "kernels/gated_ffn_f16.hip", "kernels/gated_ffn_f32.hip"]
+HEADERS = ["common.h", "token_ops.h", "kernels/gated_ffn_gemm.h", "plan.h", "options.h", "kernels/qstats.h", "kernels/epilogue.h", "kernels/rng.h", "kernels/act.h", "../../include/gddim_amd.h"]
 ARCH = "gfx950"
 # per-file flags: the split6 kernel wants its fp32 adds scalar (v_pk_add_f32 costs issue time beside bf16 MFMAs)
 # packed fp32 instructions (v_pk_add / mul / fma_f32) stay out of the token operators: some of their forms have given wrong results now and then
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-EXTRA_FLAGS = {"kernels/conv3x3_wino2d_split6.hip": ["-fno-slp-vectorize"], "token_ops.cpp": NO_PACKED_F32, "kernels/rotary.hip": NO_PACKED_F32}
+EXTRA_FLAGS = {"kernels/conv3x3_wino2d_split6.hip": ["-fno-slp-vectorize"]}
+EXTRA_FLAGS.update({src: NO_PACKED_F32 for src in SOURCES if src == "token_ops.cpp" or "rotary" in src or "gated_ffn" in src})
 
 
 def _hipcc():

@@ -1,0 +1,426 @@
+// The matrix products of the gated feed-forward block (one translation unit per element type includes this).
+//
+//   forward    h = act(x Wg^T) (.) (x Wu^T)      both projections share the tiles of x; activation and product in the epilogue
+//              y = h Wd^T
+//   backward   dh = dy Wd, and in its epilogue    dgate = dh (.) up (.) act'(gate),   dup = dh (.) act(gate)
+//              dx = dgate Wg + dup Wu              one sum over 2 F
+//              dWg = dgate^T x, dWu = dup^T x, dWd = dy^T h     one launch
+//
+// C[m][n] = sum_k A[m][k] B[n][k].  Each operand lies in memory with k adjacent (KC: x, weights as torch.nn.Linear keeps them) or with its other index
+// adjacent (the weights in dh and dx, everything in the weights' gradients); no operand is transposed in memory.
+//
+// Tiles.  A step of the k loop stages 128 bytes of k (64 16-bit or 32 float32 values) for BM rows of A and BN of B in LDS, two stages.  KC rows are 128 bytes =
+// 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  Global memory goes to LDS directly, 16 bytes a
+// lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole 16-byte pieces, through registers.
+// A fragment is 16 bytes a lane either way: row (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing
+// LDS read gathers it where k is not adjacent), one v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care
+// which k a lane holds as long as both operands agree, so both layouts and all types share one loop.
+// The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m, and stores them with one 8 / 16-byte store.
+//
+// All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type: gate, up, h (the operands of the next product must be, on the 16-bit
+// matrix core, and gate / up are what a training step keeps), dgate, dup, and the results.
+#pragma once
+#include "../common.h"
+#include "../token_ops.h"
+
+namespace gd {
+namespace ffn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct quad { typedef T type __attribute__((ext_vector_type(4))); };
+
+// ---- activation and its derivative, float32 ----
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == GD_ACT_SILU) return z / (1.f + expf(-z));
+    if (act == GD_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
+    return 0.5f * z * (1.f + t);
+}
+
+__device__ __forceinline__ void act_grad(float z, int act, float &a, float &da) {
+    if (act == GD_ACT_SILU) {
+        const float s = 1.f / (1.f + expf(-z));
+        a = z * s;
+        da = s * (1.f + z * (1.f - s));
+    } else if (act == GD_ACT_GELU) {
+        const float c = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        a = z * c;
+        da = c + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    } else {
+        const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
+        a = 0.5f * z * (1.f + t);
+        da = 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
+    }
+}
+
+// ---- epilogues on four adjacent columns of one row ----
+template <typename T> __device__ __forceinline__ void store4(void *p, long long o, f32x4 v, int n_left, bool whole) {
+    T *d = static_cast<T *>(p) + o;
+    if (whole) *reinterpret_cast<typename quad<T>::type *>(d) = __builtin_convertvector(v, typename quad<T>::type);
+    else
+        for (int i = 0; i < 4 && i < n_left; ++i) d[i] = (T)v[i];
+}
+
+template <typename T> __device__ __forceinline__ f32x4 load4(const void *p, long long o, int n_left, bool whole) {
+    const T *d = static_cast<const T *>(p) + o;
+    if (whole) return __builtin_convertvector(*reinterpret_cast<const typename quad<T>::type *>(d), f32x4);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4 && i < n_left; ++i) v[i] = (float)d[i];
+    return v;
+}
+
+// c0 (and c1: up, for EPI_GATED) of row m, columns n .. n + 3
+template <typename T, int EPI>
+__device__ __forceinline__ void epilogue4(const GemmProblem &q, int act, int m, int n, f32x4 c0, f32x4 c1) {
+    const int left = q.N - n;
+    const bool whole = q.quads && left >= 4;
+    const long long o = (long long)m * q.N + n;
+    if constexpr (EPI == EPI_STORE) store4<T>(q.out[0], o, c0, left, whole);
+    else if constexpr (EPI == EPI_GATED) {
+        f32x4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = act_value(c0[i], act) * c1[i];
+        store4<T>(q.out[0], o, h, left, whole);
+        if (q.out[1]) {
+            store4<T>(q.out[1], o, c0, left, whole);
+            store4<T>(q.out[2], o, c1, left, whole);
+        }
+    } else {
+        const f32x4 gate = load4<T>(q.in[0], o, left, whole), up = load4<T>(q.in[1], o, left, whole);
+        f32x4 dg, du;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a, da;
+            act_grad(gate[i], act, a, da);
+            dg[i] = c0[i] * up[i] * da;
+            du[i] = c0[i] * a;
+        }
+        store4<T>(q.out[0], o, dg, left, whole);
+        store4<T>(q.out[1], o, du, left, whole);
+    }
+}
+
+// ---- one 16-byte fragment each: acc += B-fragment x A-fragment ----
+template <typename T> __device__ __forceinline__ f32x4 mma(i32x4 b, i32x4 a, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mma<__bf16>(i32x4 b, i32x4 a, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mma<_Float16>(i32x4 b, i32x4 a, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mma<float>(i32x4 b, i32x4 a, f32x4 c) {
+    const f32x4 bf = __builtin_bit_cast(f32x4, b), af = __builtin_bit_cast(f32x4, a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[i], af[i], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ int kc_swizzle(int row) { return (row >> 1) & 7; }
+
+constexpr unsigned OUT_OF_RANGE = 0x80000000u;  // a buffer offset past every num_records used here: the piece arrives as zeros
+
+// One operand: R rows (of m or n) x 128 bytes of k per stage
+template <typename T, int R, bool KC, int THREADS, bool GATED_B>
+struct Operand {
+    static constexpr int ES = sizeof(T), KSTEP = 128 / ES, V = 16 / ES;   // k per stage, elements of a piece
+    static constexpr int WAVES = THREADS / 64;
+    static constexpr int PIECES = R * 8 / THREADS;                        // 16-byte pieces a thread stages
+    static constexpr int CPR = KC ? 8 : R * ES / 16;                      // pieces of an LDS row
+    static constexpr int BYTES = R * 128;
+
+    const char *base[2];   // element (first row, k = 0) of each source
+    long long end[2];      // bytes from there to the end of the matrix
+    long long ld;          // bytes
+    int k_len;             // k of one source
+    int rows_left;         // rows (KC) / columns (else) from the tile's first
+    int row[PIECES], piece[PIECES];  // of the matrix tile: KC row / k row; source piece
+
+    __device__ __forceinline__ void init(int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int slot = (i * WAVES + wave) * 64 + lane;  // 16-byte slot of the stage
+            row[i] = slot / CPR;
+            piece[i] = (slot % CPR) ^ swizzle(row[i]);
+        }
+    }
+    __device__ static __forceinline__ int swizzle(int r) {
+        if constexpr (KC) return kc_swizzle(r);
+        else if constexpr (ES == 2) return 2 * (r & 3) + 8 * ((r >> 3) & 1);
+        else return 4 * ((r >> 2) & 3);
+    }
+    // gated B tiles: rows of gate and up alternate in blocks of 32, so that a wave's 64 columns hold both of its 32
+    __device__ static __forceinline__ int source_of(int r) { return GATED_B ? (r >> 5) & 1 : 0; }
+    __device__ static __forceinline__ int row_in_source(int r) { return GATED_B ? ((r >> 6) << 5) + (r & 31) : r; }
+
+    // stage the 128 bytes of k from step kt (src: which source of a two-part sum) straight into LDS
+    __device__ __forceinline__ void stage_direct(char *lds, int src, int kt, int wave) const {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass has no buffer descriptors
+        const long long adv = KC ? (long long)kt * 128 : (long long)kt * KSTEP * ld;
+        __amdgpu_buffer_rsrc_t rs[GATED_B ? 2 : 1];
+#pragma unroll
+        for (int g = 0; g < (GATED_B ? 2 : 1); ++g) {
+            const int s = GATED_B ? g : src;
+            long long left = end[s] - adv;
+            left = left < 0 ? 0 : left > 0x7fffffffLL ? 0x7fffffffLL : left;
+            rs[g] = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base[s]) + adv, 0, (int)left, 0x00020000);
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            unsigned off;
+            bool in;
+            if constexpr (KC) {
+                off = (unsigned)row_in_source(row[i]) * (unsigned)ld + piece[i] * 16;
+                in = kt * KSTEP + piece[i] * V < k_len;
+            } else {
+                off = (unsigned)row[i] * (unsigned)ld + piece[i] * 16;
+                in = kt * KSTEP + row[i] < k_len;
+            }
+            off = in ? off : OUT_OF_RANGE;
+            const int g = GATED_B ? source_of((i * WAVES + wave) * 64 / CPR) : 0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs[g], (__attribute__((address_space(3))) void *)(lds + (i * WAVES + wave) * 1024), 16, off, 0, 0, 0);
+        }
+#endif
+    }
+    // ... through registers, for rows that are not whole aligned pieces
+    __device__ __forceinline__ void load_regs(i32x4 *r, int src, int kt) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int k0 = kt * KSTEP + (KC ? piece[i] * V : row[i]);
+            const int s = GATED_B ? source_of(row[i]) : src;
+            const int rr = KC ? row_in_source(row[i]) : piece[i] * V;  // first row / column
+            const char *p = KC ? base[s] + (long long)rr * ld + (long long)k0 * ES : base[s] + (long long)k0 * ld + (long long)rr * ES;
+            const bool line = KC ? rr < rows_left : k0 < k_len;
+            const int left = line ? (KC ? k_len - k0 : rows_left - rr) : 0;
+            r[i] = i32x4{0, 0, 0, 0};
+            if (left >= V) __builtin_memcpy(&r[i], p, 16);
+            else if (left > 0) {
+                T t[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) t[j] = j < left ? reinterpret_cast<const T *>(p)[j] : (T)0.f;
+                __builtin_memcpy(&r[i], t, 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void store_regs(char *lds, const i32x4 *r, int wave, int lane) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<i32x4 *>(lds + ((i * WAVES + wave) * 64 + lane) * 16) = r[i];
+    }
+
+    // fragment: rows r0 + lane % 16, half kk of the stage's k
+    __device__ static __forceinline__ i32x4 fragment(const char *lds, int r0, int kk, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        if constexpr (KC) {
+            const int r = r0 + i;
+            return *reinterpret_cast<const i32x4 *>(lds + r * 128 + (((kk * 4 + g) ^ kc_swizzle(r)) << 4));
+        } else if constexpr (ES == 2) {
+            typedef __attribute__((address_space(3))) i16x4 *lds_ptr;
+            i16x8 v;
+            const int k = kk * 32 + g * 8 + (i >> 2);
+            const char *p = lds + k * (R * 2) + (((r0 / 8 + ((i & 3) >> 1)) ^ swizzle(k)) << 4) + (i & 1) * 8;
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * R * 2));
+            v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(i32x4, v);
+        } else {
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = (kk * 4 + g) * 4 + j, c = r0 + i;
+                v[j] = *reinterpret_cast<const float *>(lds + k * (R * 4) + (((c >> 2) ^ swizzle(k)) << 4) + (c & 3) * 4);
+            }
+            return __builtin_bit_cast(i32x4, v);
+        }
+    }
+};
+
+// workgroup -> (problem, tile, split): workgroups go round-robin over the 8 XCDs, each with an L2 of its own; consecutive tiles of one XCD share
+// operand rows, eight m tiles to a group
+struct Place {
+    int problem, mt, nt, split;
+};
+__device__ __forceinline__ Place place(const GemmLaunch &p) {
+    const int total = gridDim.x, id = blockIdx.x;
+    const int q = total >> 3, r = total & 7, xcd = id & 7;
+    int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+    Place w;
+    w.problem = 0;
+    while (w.problem + 1 < p.problems && t >= p.q[w.problem].blocks) t -= p.q[w.problem++].blocks;
+    const GemmProblem &g = p.q[w.problem];
+    const int tiles = g.tiles_m * g.tiles_n;
+    w.split = t / tiles;
+    t -= w.split * tiles;
+    const int group = 8 * g.tiles_n;
+    const int first = t / group * 8, size = min(8, g.tiles_m - first);
+    t %= group;
+    w.mt = first + t % size;
+    w.nt = t / size;
+    return w;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool DIRECT>
+__global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p) {
+    constexpr int THREADS = WM * WN * 64;
+    constexpr bool GATED = EPI == EPI_GATED;
+    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+    static_assert(!GATED || TN == 64, "a wave's columns are 32 of gate and 32 of up");
+    typedef Operand<T, BM, AKC, THREADS, false> OpA;
+    typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
+    constexpr int STAGE = OpA::BYTES + OpB::BYTES;
+    constexpr int KSTEP = OpA::KSTEP;
+    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const Place w = place(p);
+    const GemmProblem &q = p.q[w.problem];
+    const int m0 = w.mt * BM, n0 = w.nt * (GATED ? BN / 2 : BN);
+
+    OpA a;
+    OpB b;
+    a.init(wave, lane);
+    b.init(wave, lane);
+    a.ld = q.lda; b.ld = q.ldb;
+    a.k_len = b.k_len = q.K;
+    a.rows_left = q.M - m0; b.rows_left = q.N - n0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const long long oa = AKC ? (long long)m0 * q.lda : (long long)m0 * sizeof(T);
+        const long long ob = BKC ? (long long)n0 * q.ldb : (long long)n0 * sizeof(T);
+        a.base[s] = static_cast<const char *>(q.a[s]) + oa;
+        b.base[s] = static_cast<const char *>(q.b[s]) + ob;
+        a.end[s] = q.a_bytes - oa;
+        b.end[s] = q.b_bytes - ob;
+    }
+    const int per_part = (q.K + KSTEP - 1) / KSTEP;       // steps of one part of the sum
+    const int kt0 = w.split * q.steps_per_split;
+    const int kt1 = min(kt0 + q.steps_per_split, per_part * q.parts);
+
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    i32x4 ra[DIRECT ? 1 : OpA::PIECES], rb[DIRECT ? 1 : OpB::PIECES];
+    auto fetch = [&](int kt, char *stage) __attribute__((always_inline)) {
+        const int src = kt >= per_part, k = src ? kt - per_part : kt;
+        if constexpr (DIRECT) {
+            a.stage_direct(stage, src, k, wave);
+            b.stage_direct(stage + OpA::BYTES, src, k, wave);
+        } else {
+            a.load_regs(ra, src, k);
+            b.load_regs(rb, src, k);
+        }
+    };
+    auto commit = [&](char *stage) __attribute__((always_inline)) {
+        if constexpr (!DIRECT) {
+            a.store_regs(stage, ra, wave, lane);
+            b.store_regs(stage + OpA::BYTES, rb, wave, lane);
+        }
+    };
+
+    fetch(kt0, lds);
+    commit(lds);
+    for (int kt = kt0; kt < kt1; ++kt) {
+        char *cur = lds + ((kt - kt0) & 1) * STAGE, *nxt = lds + ((kt - kt0 + 1) & 1) * STAGE;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces of the current stage are in LDS ...
+        __syncthreads();                     // ... and everyone's; the other stage has been read by all
+        if (kt + 1 < kt1) fetch(kt + 1, nxt);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            i32x4 fa[FM], fb[FN];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fa[j] = OpA::fragment(cur, wm * TM + j * 16, kk, lane);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) fb[i] = OpB::fragment(cur + OpA::BYTES, wn * TN + i * 16, kk, lane);
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = mma<T>(fb[i], fa[j], acc[i][j]);
+        }
+        if (kt + 1 < kt1) commit(nxt);
+    }
+
+    // row m of fragment column j, columns n .. n + 3 of fragment row i
+    constexpr int NI = GATED ? FN / 2 : FN;
+    const int mr = m0 + wm * TM + (lane & 15);
+    const int nr = n0 + wn * (GATED ? TN / 2 : TN) + (lane >> 4) * 4;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int m = mr + j * 16;
+        if (m >= q.M) continue;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int n = nr + i * 16;
+            if (n >= q.N) continue;
+            const f32x4 c1 = GATED ? acc[(i + NI) % FN][j] : f32x4{0.f, 0.f, 0.f, 0.f};
+            if (q.splits == 1) epilogue4<T, EPI>(q, p.act, m, n, acc[i][j], c1);
+            else {  // partial sums, rows padded to whole quads: [split][plane][M][N4]
+                const long long n4 = (q.N + 3) & ~3, plane = (long long)q.M * n4;
+                float *d = q.partial + (long long)w.split * (GATED ? 2 : 1) * plane + (long long)m * n4 + n;
+                *reinterpret_cast<f32x4 *>(d) = acc[i][j];
+                if constexpr (GATED) *reinterpret_cast<f32x4 *>(d + plane) = c1;
+            }
+        }
+    }
+}
+
+// the splits' partial sums in order, then the epilogue: one quad of columns per thread
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void join_kernel(const GemmLaunch p) {
+    constexpr bool GATED = EPI == EPI_GATED;
+    long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+    int k = 0;
+    while (k + 1 < p.problems && t >= p.q[k].join_threads) t -= p.q[k++].join_threads;
+    const GemmProblem &q = p.q[k];
+    if (q.splits == 1 || t >= q.join_threads) return;
+    const int quads = (q.N + 3) >> 2;
+    const int m = (int)(t / quads), n = (int)(t - (long long)m * quads) * 4;
+    if (m >= q.M) return;
+    const long long n4 = (long long)quads * 4, plane = (long long)q.M * n4;
+    const float *d = q.partial + (long long)m * n4 + n;
+    f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < q.splits; ++s) {
+        c0 += *reinterpret_cast<const f32x4 *>(d + (long long)s * (GATED ? 2 : 1) * plane);
+        if constexpr (GATED) c1 += *reinterpret_cast<const f32x4 *>(d + (long long)s * 2 * plane + plane);
+    }
+    epilogue4<T, EPI>(q, p.act, m, n, c0, c1);
+}
+
+template <typename T, bool AKC, bool BKC, int EPI>
+int launch_gemm(const GemmLaunch &p, int blocks, hipStream_t s) {
+    if (blocks > 0) {
+        if (p.tile == TILE_256) {
+            if constexpr (sizeof(T) == 2) gemm_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, true><<<blocks, 512, 0, s>>>(p);
+        } else if (p.direct) gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, true><<<blocks, 256, 0, s>>>(p);
+        else gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, false><<<blocks, 256, 0, s>>>(p);
+        GD_HIP(hipGetLastError());
+    }
+    if (p.join_blocks > 0) {
+        join_kernel<T, EPI><<<p.join_blocks, 256, 0, s>>>(p);
+        GD_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+template <typename T>
+int launch_type(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s) {
+    switch (kind) {
+        case GEMM_GATE_UP: return launch_gemm<T, true, true, EPI_GATED>(p, blocks, s);
+        case GEMM_DOWN: return launch_gemm<T, true, true, EPI_STORE>(p, blocks, s);
+        case GEMM_DHIDDEN: return launch_gemm<T, true, false, EPI_GATED_BWD>(p, blocks, s);
+        case GEMM_DX: return launch_gemm<T, true, false, EPI_STORE>(p, blocks, s);
+        case GEMM_DW: return launch_gemm<T, false, false, EPI_STORE>(p, blocks, s);
+    }
+    return 1;
+}
+
+}  // namespace ffn
+}  // namespace gd

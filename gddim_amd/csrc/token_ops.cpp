@@ -37,9 +37,209 @@ int view(HeadsView &v, const gd_heads *h, bool empty, const char *who, const cha
     return 0;
 }
 
+// ---- gated feed-forward block ----
+size_t elem_size(int dtype) { return dtype == GD_F32 ? 4 : 2; }
+
+int check_ffn(const gd_ffn_desc *d, const char *who) {
+    GD_CHECK(d, "%s: null description", who);
+    GD_CHECK(d->dtype == GD_F32 || d->dtype == GD_BF16 || d->dtype == GD_F16, "%s: unknown element type %d", who, d->dtype);
+    GD_CHECK(d->act == GD_ACT_SILU || d->act == GD_ACT_GELU || d->act == GD_ACT_GELU_TANH, "%s: unknown activation %d", who, d->act);
+    GD_CHECK(d->rows >= 0 && d->in >= 1 && d->hidden >= 1 && d->out >= 1, "%s: bad sizes rows=%d in=%d hidden=%d out=%d", who, d->rows, d->in, d->hidden, d->out);
+    const long long most = 1LL << 30;
+    GD_CHECK(d->rows <= most && d->in <= most && d->hidden <= most && d->out <= most, "%s: sizes past 2^30", who);
+    GD_CHECK((d->rows <= 1 || d->ld_x >= d->in) && (d->hidden <= 1 || d->ld_w_in >= d->in) && (d->out <= 1 || d->ld_w_down >= d->hidden),
+             "%s: a leading dimension is shorter than its row", who);
+    return 0;
+}
+
+struct Matrix {
+    const void *p;
+    long long rows, cols, ld;  // elements
+};
+
+bool pieces_ok(const Matrix &m, bool k_adjacent, size_t es) {
+    const long long ld = m.ld * (long long)es;
+    return (uintptr_t)m.p % 16 == 0 && ld % 16 == 0 && ld <= (1LL << 22) && (!k_adjacent || m.cols * (long long)es % 16 == 0);
+}
+
+// C (M, N) = sum of parts A B; operands as they lie in memory, k adjacent or not
+GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int parts, bool gated, size_t es, int *direct) {
+    GemmProblem q{};
+    q.M = (int)(akc ? a[0].rows : a[0].cols);
+    q.N = (int)(bkc ? b[0].rows : b[0].cols);
+    q.K = (int)(akc ? a[0].cols : a[0].rows);
+    q.parts = parts;
+    auto bytes = [&](const Matrix &m) { return m.rows ? ((m.rows - 1) * m.ld + m.cols) * (long long)es : 0; };
+    q.lda = a[0].ld * es; q.ldb = b[0].ld * es;
+    q.a_bytes = bytes(a[0]); q.b_bytes = bytes(b[0]);
+    for (int s = 0; s < 2; ++s) {
+        const Matrix &ma = a[parts == 2 ? s : 0], &mb = b[parts == 2 || gated ? s : 0];
+        q.a[s] = ma.p; q.b[s] = mb.p;
+        if (!pieces_ok(ma, akc, es) || !pieces_ok(mb, bkc, es)) *direct = 0;
+    }
+    return q;
+}
+
+// tile and split of a launch; returns the floats of partial sums it needs, or -1 (more workgroups than a grid holds)
+long long plan_gemm(GemmLaunch &l, int dtype, bool gated) {
+    const long long cus = device_cus();
+    const int kstep = 128 / (int)elem_size(dtype);
+    auto tiles = [&](int t) {
+        long long n = 0;
+        for (int i = 0; i < l.problems; ++i) n += ((l.q[i].M + t - 1LL) / t) * ((l.q[i].N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
+        return n;
+    };
+    // 256 x 256 tiles read half the LDS bytes per product of 128 x 128 ones, but one workgroup holds a CU: taken where they fill most of the chip
+    l.tile = dtype != GD_F32 && l.direct && 4 * tiles(256) >= 3 * cus ? TILE_256 : TILE_128;
+    const int t = l.tile == TILE_256 ? 256 : 128;
+    const long long all = tiles(t), room = l.tile == TILE_256 ? cus : 2 * cus;
+    if (all > (1LL << 30)) return -1;
+    long long floats = 0, join = 0, blocks = 0;
+    for (int i = 0; i < l.problems; ++i) {
+        GemmProblem &q = l.q[i];
+        q.tiles_m = (int)((q.M + t - 1LL) / t);
+        q.tiles_n = (int)((q.N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
+        const long long steps = (long long)q.parts * ((q.K + kstep - 1) / kstep);
+        // few tiles and a long sum: split it over workgroups, at least 4 steps each
+        long long splits = all > 0 ? room / all : 1;
+        if (splits > steps / 4) splits = steps / 4;
+        if (splits > 16) splits = 16;
+        if (splits < 1) splits = 1;
+        q.steps_per_split = (int)((steps + splits - 1) / splits);
+        q.splits = q.steps_per_split ? (int)((steps + q.steps_per_split - 1) / q.steps_per_split) : 1;
+        q.blocks = q.tiles_m * q.tiles_n * q.splits;
+        blocks += q.blocks;
+        q.join_threads = 0;
+        if (q.splits > 1) {
+            const long long n4 = (q.N + 3LL) / 4 * 4;
+            q.join_threads = ((long long)q.M * (n4 / 4) + 255) / 256 * 256;
+            floats += (long long)q.splits * (gated ? 2 : 1) * q.M * n4;
+        }
+        join += q.join_threads;
+    }
+    if (blocks > (1LL << 30) || join / 256 > (1LL << 30)) return -1;
+    l.join_blocks = (int)(join / 256);
+    return floats;
+}
+
+int run_gemm(GemmLaunch &l, int dtype, GemmKind kind, float *partial, hipStream_t s, const char *who) {
+    const bool gated = kind == GEMM_GATE_UP;
+    GD_CHECK(plan_gemm(l, dtype, gated) >= 0, "%s: too many tiles for one launch", who);
+    int blocks = 0;
+    for (int i = 0; i < l.problems; ++i) {
+        GemmProblem &q = l.q[i];
+        q.quads = q.N % 4 == 0;
+        for (const void *o : {(const void *)q.out[0], (const void *)q.out[1], (const void *)q.out[2], q.in[0], q.in[1]})
+            if ((uintptr_t)o % (4 * elem_size(dtype))) q.quads = 0;
+        q.partial = partial;
+        if (q.splits > 1) partial += (long long)q.splits * (gated ? 2 : 1) * q.M * ((q.N + 3LL) / 4 * 4);
+        blocks += q.blocks;
+    }
+    switch (dtype) {
+        case GD_BF16: return launch_ffn_gemm_bf16(l, kind, blocks, s);
+        case GD_F16: return launch_ffn_gemm_f16(l, kind, blocks, s);
+        default: return launch_ffn_gemm_f32(l, kind, blocks, s);
+    }
+}
+
+struct FfnLaunches {
+    GemmLaunch l[5];  // by GemmKind
+};
+
+// the block's five launches, without what is only known at the call (outputs); null pointers count as aligned
+FfnLaunches ffn_launches(const gd_ffn_desc *d, const void *x, const void *wg, const void *wu, const void *wd, const void *hidden, const void *dy,
+                         long long ld_dy, const void *dgate, const void *dup) {
+    const size_t es = elem_size(d->dtype);
+    const Matrix X{x, d->rows, d->in, d->ld_x}, Wg{wg, d->hidden, d->in, d->ld_w_in}, Wu{wu, d->hidden, d->in, d->ld_w_in},
+        Wd{wd, d->out, d->hidden, d->ld_w_down}, H{hidden, d->rows, d->hidden, d->hidden}, DY{dy, d->rows, d->out, ld_dy},
+        DG{dgate, d->rows, d->hidden, d->hidden}, DU{dup, d->rows, d->hidden, d->hidden};
+    FfnLaunches f{};
+    for (auto &l : f.l) { l.problems = 1; l.direct = 1; l.act = d->act; }
+    const Matrix w_in[2] = {Wg, Wu}, d_in[2] = {DG, DU};
+    f.l[GEMM_GATE_UP].q[0] = problem(&X, true, w_in, true, 1, true, es, &f.l[GEMM_GATE_UP].direct);
+    f.l[GEMM_DOWN].q[0] = problem(&H, true, &Wd, true, 1, false, es, &f.l[GEMM_DOWN].direct);
+    f.l[GEMM_DHIDDEN].q[0] = problem(&DY, true, &Wd, false, 1, false, es, &f.l[GEMM_DHIDDEN].direct);
+    f.l[GEMM_DX].q[0] = problem(d_in, true, w_in, false, 2, false, es, &f.l[GEMM_DX].direct);
+    GemmLaunch &w = f.l[GEMM_DW];
+    w.problems = 3;
+    w.q[0] = problem(&DG, false, &X, false, 1, false, es, &w.direct);
+    w.q[1] = problem(&DU, false, &X, false, 1, false, es, &w.direct);
+    w.q[2] = problem(&DY, false, &H, false, 1, false, es, &w.direct);
+    return f;
+}
+
+long long align_up(long long n) { return (n + 255) / 256 * 256; }
+
+// floats of partial sums any of the given launches may need, whatever the alignment of the tensors turns out to be
+long long partial_floats(FfnLaunches f, int dtype, int first, int last) {
+    long long most = 0;
+    for (int k = first; k <= last; ++k)
+        for (int direct = 0; direct < 2; ++direct) {
+            GemmLaunch l = f.l[k];
+            l.direct = direct;
+            const long long n = plan_gemm(l, dtype, k == GEMM_GATE_UP);
+            if (n > most) most = n;
+        }
+    return most;
+}
+
 }  // namespace
 
 extern "C" {
+
+long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward) {
+    if (check_ffn(d, "gated_ffn_workspace")) return -1;
+    const FfnLaunches f = ffn_launches(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, d->out, nullptr, nullptr);
+    if (!backward) return partial_floats(f, d->dtype, GEMM_GATE_UP, GEMM_DOWN) * (long long)sizeof(float);
+    const long long grad = align_up((long long)d->rows * d->hidden * (long long)elem_size(d->dtype));
+    return 2 * grad + partial_floats(f, d->dtype, GEMM_DHIDDEN, GEMM_DW) * (long long)sizeof(float);
+}
+
+int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, void *gate_dev, void *up_dev,
+                 void *hidden_dev, void *y, void *workspace_dev, void *stream) {
+    static const char *who = "gated_ffn";
+    GD_TRY(check_ffn(d, who));
+    const bool empty = d->rows == 0;
+    GD_CHECK(w_gate && w_up && w_down && (empty || (x && hidden_dev && y)), "%s: null pointer", who);
+    GD_CHECK(!gate_dev == !up_dev, "%s: gate and up are kept both or neither", who);
+    if (empty) return 0;
+    GD_CHECK((uintptr_t)workspace_dev % 16 == 0, "%s: workspace not aligned to 16 bytes", who);
+    GD_CHECK(workspace_dev || gd_gated_ffn_workspace(d, 0) == 0, "%s: null workspace", who);
+    FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden_dev, nullptr, d->out, nullptr, nullptr);
+    GemmLaunch &g = f.l[GEMM_GATE_UP], &o = f.l[GEMM_DOWN];
+    g.q[0].out[0] = hidden_dev; g.q[0].out[1] = gate_dev; g.q[0].out[2] = up_dev;
+    o.q[0].out[0] = y;
+    GD_TRY(run_gemm(g, d->dtype, GEMM_GATE_UP, static_cast<float *>(workspace_dev), (hipStream_t)stream, who));
+    return run_gemm(o, d->dtype, GEMM_DOWN, static_cast<float *>(workspace_dev), (hipStream_t)stream, who);
+}
+
+int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy, const void *x, const void *w_gate, const void *w_up,
+                          const void *w_down, const void *gate, const void *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
+                          void *dw_down, void *workspace_dev, void *stream) {
+    static const char *who = "gated_ffn_backward";
+    GD_TRY(check_ffn(d, who));
+    const bool empty = d->rows == 0;
+    GD_CHECK(w_gate && w_up && w_down && dw_gate && dw_up && dw_down && (empty || (dy && x && gate && up && hidden && dx && workspace_dev)), "%s: null pointer", who);
+    GD_CHECK(d->rows <= 1 || ld_dy >= d->out, "%s: a leading dimension is shorter than its row", who);
+    GD_CHECK((uintptr_t)workspace_dev % 16 == 0, "%s: workspace not aligned to 16 bytes", who);
+    const long long grad = align_up((long long)d->rows * d->hidden * (long long)elem_size(d->dtype));
+    char *ws = static_cast<char *>(workspace_dev);
+    void *dgate = ws, *dup = ws ? ws + grad : nullptr;
+    float *partial = reinterpret_cast<float *>(ws ? ws + 2 * grad : nullptr);
+    FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden, dy, ld_dy, dgate, dup);
+    hipStream_t s = (hipStream_t)stream;
+    if (!empty) {
+        GemmProblem &h = f.l[GEMM_DHIDDEN].q[0];
+        h.out[0] = dgate; h.out[1] = dup;
+        h.in[0] = gate; h.in[1] = up;
+        GD_TRY(run_gemm(f.l[GEMM_DHIDDEN], d->dtype, GEMM_DHIDDEN, partial, s, who));
+        f.l[GEMM_DX].q[0].out[0] = dx;
+        GD_TRY(run_gemm(f.l[GEMM_DX], d->dtype, GEMM_DX, partial, s, who));
+    }
+    GemmLaunch &w = f.l[GEMM_DW];
+    w.q[0].out[0] = dw_gate; w.q[1].out[0] = dw_up; w.q[2].out[0] = dw_down;
+    return run_gemm(w, d->dtype, GEMM_DW, partial, s, who);
+}
 
 int gd_rotary(const gd_rotary_desc *d, const gd_heads *x, const gd_heads *out, int heads, int inverse, void *stream) {
     RotaryParams p{};

@@ -43,4 +43,35 @@ struct RotaryParams {
 enum RotaryMode { ROT_PLAIN = 0, ROT_NORM = 1, ROT_NORM_BWD = 2 };
 int launch_rotary(RotaryParams p, int dtype, RotaryMode mode, void *dw0, void *dw1, hipStream_t s);
 
+// ---- gated feed-forward block (kernels/gated_ffn_gemm.h) ----
+enum GemmKind { GEMM_GATE_UP, GEMM_DOWN, GEMM_DHIDDEN, GEMM_DX, GEMM_DW };
+enum GemmEpilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD };
+enum GemmTile { TILE_128, TILE_256 };
+
+// C[m][n] = sum over parts and k of A[m][k] B[n][k]
+struct GemmProblem {
+    const void *a[2], *b[2];     // two-part sums: a[1], b[1]; GEMM_GATE_UP: b = {Wg, Wu}
+    long long lda, ldb;          // bytes from row to row of the matrix as it lies in memory
+    long long a_bytes, b_bytes;  // extent of a matrix in memory
+    int M, N, K, parts;
+    void *out[3];                // rows of N elements, dense
+    const void *in[2];           // EPI_GATED_BWD: gate, up
+    int quads;                   // N % 4 == 0 and outputs aligned: four columns per store
+    int splits, steps_per_split;
+    float *partial;
+    // filled in by the launcher
+    int tiles_m, tiles_n, blocks;
+    long long join_threads;
+};
+
+struct GemmLaunch {
+    GemmProblem q[3];
+    int problems, act, direct, join_blocks;
+    GemmTile tile;
+};
+
+int launch_ffn_gemm_bf16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
+int launch_ffn_gemm_f16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
+int launch_ffn_gemm_f32(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
+
 }  // namespace gd

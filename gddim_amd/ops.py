@@ -5,7 +5,7 @@ import ctypes
 
 from . import _abi
 from ._abi import GddimError, check
-from .token_ops import RotaryAxes, qk_norm_rotary, qk_norm_rotary_backward, rotary  # noqa: F401
+from .token_ops import RotaryAxes, gated_ffn, gated_ffn_backward, qk_norm_rotary, qk_norm_rotary_backward, rotary  # noqa: F401
 
 
 def _need_gpu(t):

@@ -8,7 +8,7 @@ import ctypes
 import math
 
 from . import _abi
-from ._abi import GddimError, Heads, RotaryDesc, check
+from ._abi import FfnDesc, GddimError, Heads, RotaryDesc, check
 
 _TORCH = None
 
@@ -220,3 +220,93 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes,
                                              _w_f32(q, w_q, w_k), float(eps), ws.data_ptr(),
                                              dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None, stream))
     return dq, dk, dwq, dwk
+
+
+# ---- gated feed-forward block ------------------------------------------------------------------------------------------------
+_ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def _rows(t, columns):
+    """t (..., columns) as a matrix with adjacent columns and rows at least a row apart: a view where there is one"""
+    t = t.reshape(-1, columns)
+    if (columns > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < columns):
+        t = t.contiguous()
+    return t
+
+
+def _check_ffn(x, w_gate, w_up, w_down, act):
+    _on_gpu(x, "x")
+    if act not in _ACTS:
+        raise GddimError("act=%r, expected one of %s" % (act, sorted(_ACTS)))
+    if x.dtype not in _torch()[1]:
+        raise GddimError("x is %s; float32, bfloat16 and float16 are supported" % x.dtype)
+    for w, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
+        _like(w, name, x, "x")
+        if w.dim() != 2:
+            raise GddimError("%s has shape %s, expected two dimensions" % (name, tuple(w.shape)))
+    if x.dim() < 1 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0] or 0 in w_gate.shape or w_down.shape[0] == 0:
+        raise GddimError("x %s, w_gate %s, w_up %s, w_down %s do not fit (..., in), (hidden, in), (hidden, in), (out, hidden)" % (
+            tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
+    w_gate, w_up, w_down = _rows(w_gate, w_gate.shape[1]), _rows(w_up, w_up.shape[1]), _rows(w_down, w_down.shape[1])
+    if w_gate.stride(0) != w_up.stride(0):
+        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    x2 = _rows(x, x.shape[-1])
+    if max(x2.shape[0], *w_gate.shape, w_down.shape[0]) > 1 << 30:
+        raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (x2.shape[0], x2.shape[1], w_gate.shape[0], w_down.shape[0]))
+    desc = FfnDesc(_torch()[1][x.dtype], _ACTS[act], x2.shape[0], x2.shape[1], w_gate.shape[0], w_down.shape[0], x2.stride(0), w_gate.stride(0),
+                   w_down.stride(0))
+    return x2, w_gate, w_up, w_down, desc
+
+
+def _workspace(desc, backward, device):
+    n = _abi.lib().gd_gated_ffn_workspace(desc, backward)
+    if n < 0:
+        check(1)
+    return _torch()[0].empty(n, dtype=_torch()[0].uint8, device=device) if n else None
+
+
+def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
+    """Gated feed-forward block (act(x w_gate^T) * (x w_up^T)) w_down^T: x (..., in), weights as torch.nn.Linear keeps them -- w_gate and w_up
+    (hidden, in), w_down (out, hidden) -- act 'silu', 'gelu' or 'gelu_tanh'.  Returns y (..., out); with save=True (y, saved), saved for
+    gated_ffn_backward.  Both projections, the activation and the product are one kernel."""
+    torch = _torch()[0]
+    shape = x.shape[:-1] if isinstance(x, torch.Tensor) else ()
+    x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
+    M, F = x.shape[0], w_gate.shape[0]
+    y = torch.empty((M, w_down.shape[0]), dtype=x.dtype, device=x.device)
+    hidden = torch.empty((M, F), dtype=x.dtype, device=x.device)
+    gate, up = (torch.empty_like(hidden), torch.empty_like(hidden)) if save else (None, None)
+    with _Device(x) as stream:
+        ws = _workspace(desc, 0, x.device)
+        check(_abi.lib().gd_gated_ffn(desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
+                                      up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws.data_ptr() if ws is not None else None, stream))
+    y = y.view(*shape, w_down.shape[0])
+    return (y, (gate, up, hidden)) if save else y
+
+
+def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
+    """Gradients (dx, dw_gate, dw_up, dw_down) of gated_ffn from that of its result and what the call with save=True kept (left as it was).  The
+    same bits every time."""
+    torch = _torch()[0]
+    shape = x.shape if isinstance(x, torch.Tensor) else ()
+    x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
+    M, D, F, O = x.shape[0], x.shape[1], w_gate.shape[0], w_down.shape[0]
+    _like(dy, "dy", x, "x")
+    if tuple(dy.shape) != tuple(shape[:-1]) + (O,):
+        raise GddimError("dy has shape %s, expected %s" % (tuple(dy.shape), tuple(shape[:-1]) + (O,)))
+    if not isinstance(saved, tuple) or len(saved) != 3:
+        raise GddimError("saved: expected the second result of gated_ffn(..., save=True)")
+    for t, name in zip(saved, ("gate", "up", "hidden")):
+        _like(t, "saved " + name, x, "x")
+        if tuple(t.shape) != (M, F) or not t.is_contiguous():
+            raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
+    dy = _rows(dy, O)
+    gate, up, hidden = saved
+    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)
+    dx, dwg, dwu, dwd = new(M, D), new(F, D), new(F, D), new(O, F)
+    with _Device(x) as stream:
+        ws = _workspace(desc, 1, x.device)
+        check(_abi.lib().gd_gated_ffn_backward(desc, dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+                                               gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(),
+                                               dwd.data_ptr(), ws.data_ptr() if ws is not None else None, stream))
+    return dx.view(shape), dwg, dwu, dwd

@@ -361,6 +361,9 @@ int gd_attention_block_fused(const float *q_dev, const float *k_dev, const float
 #define GD_POS_I64 1
 #define GD_POS_F32 2
 #define GD_MAX_AXES 4
+#define GD_ACT_SILU 0
+#define GD_ACT_GELU 1      /* z Phi(z) */
+#define GD_ACT_GELU_TANH 2 /* its tanh form */
 /* one (B, N, heads, D) tensor: strides in elements, the D channels of a head adjacent; heads may be 0 in none of the calls below */
 typedef struct gd_heads {
     void *data;
@@ -390,6 +393,23 @@ long long gd_qk_norm_rotary_backward_workspace(int head_dim);
 int gd_qk_norm_rotary_backward(const gd_rotary_desc *d, const gd_heads *dq_out, const gd_heads *dk_out, const gd_heads *q, const gd_heads *k,
                                const gd_heads *dq, const gd_heads *dk, int heads_q, int heads_k, const void *w_q, const void *w_k, int w_f32,
                                float eps, void *workspace_dev, void *dw_q, void *dw_k, void *stream);
+/* Gated feed-forward block on `rows` tokens:  y = (act(x w_gate^T) (.) (x w_up^T)) w_down^T,  x (rows, in), w_gate and w_up (hidden, in),
+ * w_down (out, hidden), y (rows, out); act: GD_ACT_*.  Leading dimensions in elements (w_gate and w_up share one). */
+typedef struct gd_ffn_desc {
+    int dtype, act;
+    int rows, in, hidden, out;
+    long long ld_x, ld_w_in, ld_w_down;
+} gd_ffn_desc;
+/* hidden_dev (rows, hidden) receives act(gate) (.) up; gate_dev and up_dev (rows, hidden) the projections, or both null: what the backward call
+ * needs of a training step.  workspace_dev: gd_gated_ffn_workspace(d, 0) bytes (may be 0), 16-byte aligned. */
+long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward);
+int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, void *gate_dev, void *up_dev,
+                 void *hidden_dev, void *y, void *workspace_dev, void *stream);
+/* Gradients from dy (rows, out; rows ld_dy apart) and what the forward call kept: dx (rows, in), dw_gate, dw_up (hidden, in), dw_down (out, hidden), all
+ * dense.  workspace_dev: gd_gated_ffn_workspace(d, 1) bytes, 16-byte aligned.  The same bits every time. */
+int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy, const void *x, const void *w_gate, const void *w_up,
+                          const void *w_down, const void *gate, const void *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
+                          void *dw_down, void *workspace_dev, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,204 @@
+"""GPU tests of the gated feed-forward block and its gradients against float64 (bounds carried through every rounding: tests/token_reference.py)."""
+import pytest
+import torch
+
+import token_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def dev(native_lib):
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    return torch.device("cuda", 0)
+
+
+def _inputs(dev, M, D, F, O, dtype, seed=0):
+    g = torch.Generator(dev).manual_seed(seed)
+    n = lambda *s, scale=1.0: (torch.randn(s, generator=g, device=dev) * scale).to(dtype)
+    return n(M, D), n(F, D, scale=D ** -0.5), n(F, D, scale=D ** -0.5), n(O, F, scale=F ** -0.5), n(M, O)
+
+
+def _check(got, want, what):
+    got = got.double()
+    assert got.shape == want.val.shape, (what, got.shape, want.val.shape)
+    bad = ~((got - want.val).abs() <= want.err)
+    assert not bad.any(), "%s: %d of %d outside their bound, worst %.2f of it, first at %s" % (
+        what, int(bad.sum()), bad.numel(), float(((got - want.val).abs() / want.err).max()), bad.nonzero()[0].tolist())
+
+
+def _run(x, wg, wu, wd, dy, kind):
+    from gddim_amd import ops
+    y, saved = ops.gated_ffn(x, wg, wu, wd, act=kind, save=True)
+    return (y,) + ops.gated_ffn_backward(dy, x, wg, wu, wd, saved, act=kind)
+
+
+SIZES = [
+    # M, D, F, O
+    (1, 1, 1, 1), (1, 64, 64, 64), (1, 512, 96, 40), (2, 8, 16, 8), (3, 40, 72, 24), (5, 33, 17, 9), (16, 128, 256, 128), (17, 136, 88, 264),
+    (31, 7, 130, 3), (33, 256, 344, 256), (64, 72, 520, 72), (65, 100, 30, 101), (130, 64, 129, 66), (257, 200, 136, 96), (300, 96, 700, 250),
+    (1000, 24, 24, 24), (12, 1032, 24, 16), (700, 16, 1032, 8),
+]
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_forward_and_gradients(dev, size, typ):
+    from gddim_amd import ops
+    kind = ("silu", "gelu", "gelu_tanh")[SIZES.index(size) % 3]
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ])
+    want = ref.gated_ffn(x, wg, wu, wd, kind, TYPES[typ], dy)
+    got = _run(x, wg, wu, wd, dy, kind)
+    for g, w, what in zip(got, want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        assert g.dtype == TYPES[typ]
+        _check(g, w, what)
+    assert torch.equal(ops.gated_ffn(x, wg, wu, wd, act=kind), got[0])
+    for a, b in zip(got, _run(x, wg, wu, wd, dy, kind)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("typ", ["f32", "bf16", "f16"])
+def test_activations_over_their_range(dev, typ, kind):
+    """projections from -30 to 30, where exponentials over- and underflow"""
+    x, wg, wu, wd, dy = _inputs(dev, 70, 16, 40, 24, TYPES[typ], 3)
+    x = x * torch.linspace(0, 12, 70, device=dev, dtype=torch.float32)[:, None].to(x.dtype)
+    want = ref.gated_ffn(x, wg, wu, wd, kind, TYPES[typ], dy)
+    for g, w, what in zip(_run(x, wg, wu, wd, dy, kind), want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+@pytest.mark.parametrize("size", [(4100, 72, 1560, 64), (4100, 2888, 136, 2888), (264, 2888, 1288, 2888), (8200, 64, 264, 1352)], ids=str)
+def test_tiles_that_fill_the_chip(dev, size, typ):
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ], 1)
+    want = ref.gated_ffn(x, wg, wu, wd, "silu", TYPES[typ], dy)
+    for g, w, what in zip(_run(x, wg, wu, wd, dy, "silu"), want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+def test_strides_and_batches(dev, typ):
+    """rows and weights seen through larger matrices, both projections packed, channels not adjacent, batches of any rank, rows off any alignment"""
+    from gddim_amd import ops
+    dtype, M, D, F, O = TYPES[typ], 30, 48, 56, 40
+    x, wg, wu, wd, dy = _inputs(dev, M, D, F, O, dtype, 5)
+    want = ref.gated_ffn(x, wg, wu, wd, "gelu", dtype, dy)
+    nan = lambda *s: torch.full(s, float("nan"), dtype=dtype, device=dev)
+    packed = torch.cat((wg, wu))
+    wide_x, wide_w, wide_y = nan(M + 2, D + 16), nan(O + 1, F + 8), nan(M, O + 3)
+    wide_x[1:M + 1, 8:8 + D], wide_w[:O, :F], wide_y[:, 1:1 + O] = x, wd, dy
+    forms = [
+        (wide_x[1:M + 1, 8:8 + D], packed[:F], packed[F:], wide_w[:O, :F], wide_y[:, 1:1 + O]),
+        (x.t().contiguous().t(), wg.t().contiguous().t(), wu, wd.t().contiguous().t(), dy.t().contiguous().t()),
+        (x.view(2, 3, 5, D), wg, wu, wd, dy.view(2, 3, 5, O)),
+    ]
+    odd = nan(M * (D + 1) + 1)[1:].view(M, D + 1)
+    odd[:, :D] = x
+    forms.append((odd[:, :D], wg, wu, wd, dy))
+    for i, f in enumerate(forms):
+        got = _run(*f, "gelu")
+        assert got[0].shape == f[0].shape[:-1] + (O,) and got[1].shape == f[0].shape
+        for g, w, what in zip(got, want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+            _check(g.reshape(w.val.shape), w, "%s of form %d" % (what, i))
+    one = x[:1].expand(M, D)  # one row seen as many
+    _check(ops.gated_ffn(one, wg, wu, wd, act="gelu"), ref.gated_ffn(one, wg, wu, wd, "gelu", dtype), "expanded")
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("M", [1, 7, 40, 200])
+def test_infinities_and_nan_stay_in_their_row(dev, typ, M):
+    from gddim_amd import ops
+    x, wg, wu, wd, dy = _inputs(dev, M + 2, 72, 80, 64, TYPES[typ], 6)
+    clean = ops.gated_ffn(x, wg, wu, wd)
+    bad = x.clone()
+    bad[0] = float("nan")
+    bad[M + 1, 3] = float("inf")
+    got = ops.gated_ffn(bad, wg, wu, wd)
+    assert torch.isnan(got[0]).all() and not torch.isfinite(got[M + 1]).all()
+    assert torch.equal(got[1:M + 1], clean[1:M + 1])
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+def test_gradients_against_differences(dev, typ):
+    """a directional difference of the float64 form, step 1e-6: its own error is under 1e-8 of the sums' magnitude, the kernels' under their types' bounds"""
+    dtype = TYPES[typ]
+    x, wg, wu, wd, dy = _inputs(dev, 9, 24, 40, 16, dtype, 7)
+    got = _run(x, wg, wu, wd, dy, "gelu_tanh")
+    want = ref.gated_ffn(x, wg, wu, wd, "gelu_tanh", dtype, dy)
+    leaves = [t.double() for t in (x, wg, wu, wd)]
+    loss = lambda l: (ref.product(ref.act(ref.product(ref.V(l[0]), ref.V(l[1])), "gelu_tanh")[0] * ref.product(ref.V(l[0]), ref.V(l[2])), ref.V(l[3])).val * dy.double()).sum()
+    for i in range(4):
+        d = torch.randn(leaves[i].shape, generator=torch.Generator(dev).manual_seed(i), device=dev, dtype=torch.float64)
+        up, dn = list(leaves), list(leaves)
+        up[i], dn[i] = leaves[i] + 1e-6 * d, leaves[i] - 1e-6 * d
+        num = (loss(up) - loss(dn)) / 2e-6
+        assert abs(float(num - (got[i + 1].double() * d).sum())) <= float((want[i + 1].err * d.abs()).sum()) + 1e-6
+
+
+def test_no_rows(dev):
+    from gddim_amd import ops
+    for dtype in TYPES.values():
+        _, wg, wu, wd, _ = _inputs(dev, 1, 24, 40, 16, dtype)
+        x, dy = torch.empty(0, 24, dtype=dtype, device=dev), torch.empty(0, 16, dtype=dtype, device=dev)
+        y, saved = ops.gated_ffn(x, wg, wu, wd, save=True)
+        assert y.shape == (0, 16)
+        dx, *dw = ops.gated_ffn_backward(dy, x, wg, wu, wd, saved)
+        assert dx.shape == (0, 24) and all((g == 0).all() for g in dw)
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_other_streams_and_graph_replays(dev, M):
+    x, wg, wu, wd, dy = _inputs(dev, M, 64, 136, 64, torch.bfloat16, 8)
+    eager = _run(x, wg, wu, wd, dy, "silu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = _run(x, wg, wu, wd, dy, "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, other))
+    graphs = []
+    for _ in range(2):  # two captured calls: workspaces of their own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, _run(x, wg, wu, wd, dy, "silu")))
+        graphs[-1] = (graph, graphs[-1][1])
+    for trial in range(4):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(dev).manual_seed(trial), device=dev).to(x.dtype))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        now = _run(x, wg, wu, wd, dy, "silu")
+        for _, captured in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(now, captured))
+
+
+def test_refusals_on_the_gpu(dev):
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    x, wg, wu, wd, dy = _inputs(dev, 6, 24, 40, 16, torch.float32)
+    y, saved = ops.gated_ffn(x, wg, wu, wd, save=True)
+    bad = [
+        lambda: ops.gated_ffn(x, wg, wu, wd, act="relu"),
+        lambda: ops.gated_ffn(x.double(), wg.double(), wu.double(), wd.double()),
+        lambda: ops.gated_ffn(x, wg.half(), wu, wd),
+        lambda: ops.gated_ffn(x, wg.cpu(), wu, wd),
+        lambda: ops.gated_ffn(x, wg[:8], wu, wd),
+        lambda: ops.gated_ffn(x[:, :8], wg, wu, wd),
+        lambda: ops.gated_ffn(x, wg, wu, wd[:, :8]),
+        lambda: ops.gated_ffn(x, wg[None], wu[None], wd),
+        lambda: ops.gated_ffn(x, wg[:0], wu[:0], wd[:, :0]),
+        lambda: ops.gated_ffn(x, wg.clone().requires_grad_(), wu, wd),
+        lambda: ops.gated_ffn_backward(dy[:3], x, wg, wu, wd, saved),
+        lambda: ops.gated_ffn_backward(dy, x, wg, wu, wd, saved[:2]),
+        lambda: ops.gated_ffn_backward(dy, x, wg, wu, wd, y),
+        lambda: ops.gated_ffn_backward(dy, x, wg, wu, wd, tuple(t[:3] for t in saved)),
+        lambda: ops.gated_ffn_backward(dy.half(), x, wg, wu, wd, saved),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(GddimError):
+            call()
+            pytest.fail("call %d was not refused" % i)

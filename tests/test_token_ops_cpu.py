@@ -86,3 +86,61 @@ def test_float64_forms_against_autograd(paired):
     assert (got[0] - dx).abs().max() < 1e-12 and (got[2] - dw).abs().max() < 1e-12
     out = ref.norm_rotary(x, w, phi, (4, 8), paired, 1e-3)[0]
     assert (out[..., ia] - z.real).abs().max() < 1e-12 and (out[..., ib] - z.imag).abs().max() < 1e-12
+
+
+def _ffn(**kw):
+    from gddim_amd._abi import FfnDesc
+    d = dict(dtype=1, act=0, rows=4, in_=8, hidden=16, out=8, ld_x=8, ld_w_in=8, ld_w_down=16)
+    d.update(kw)
+    return FfnDesc(**d)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=3), dict(act=3), dict(act=-1), dict(rows=-1), dict(in_=0), dict(hidden=0), dict(out=0), dict(ld_x=7), dict(ld_w_in=7),
+                                 dict(ld_w_down=15), dict(rows=(1 << 30) + 1)], ids=str)
+def test_c_gated_ffn_refuses_descriptions(native_lib, bad):
+    d = _ffn(**bad)
+    assert native_lib.gd_gated_ffn_workspace(d, 0) == -1 and native_lib.gd_gated_ffn_workspace(d, 1) == -1
+    assert native_lib.gd_gated_ffn(d, 64, 64, 64, 64, None, None, 64, 64, 64, None) != 0
+    assert native_lib.gd_gated_ffn_backward(d, 64, 8, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None) != 0
+
+
+def test_c_gated_ffn_refuses_arguments(native_lib):
+    d = _ffn()
+    for null in range(4):
+        args = [64] * 4
+        args[null] = None
+        assert native_lib.gd_gated_ffn(d, *args, None, None, 64, 64, 64, None) != 0
+    assert native_lib.gd_gated_ffn(None, 64, 64, 64, 64, None, None, 64, 64, 64, None) != 0
+    assert native_lib.gd_gated_ffn(d, 64, 64, 64, 64, 64, None, 64, 64, 64, None) != 0   # gate without up
+    assert native_lib.gd_gated_ffn(d, 64, 64, 64, 64, None, None, None, 64, 64, None) != 0
+    assert native_lib.gd_gated_ffn(d, 64, 64, 64, 64, None, None, 64, 64, 72, None) != 0  # workspace off its alignment
+    assert native_lib.gd_gated_ffn_backward(d, 64, 7, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None) != 0
+    assert native_lib.gd_gated_ffn_backward(d, 64, 8, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None, None) != 0
+    assert native_lib.gd_gated_ffn(_ffn(rows=0), None, 64, 64, 64, None, None, None, None, None, None) == 0  # no rows: nothing is launched
+    assert native_lib.gd_gated_ffn_workspace(d, 1) >= 2 * 4 * 16 * 2
+
+
+def test_gated_ffn_needs_a_gpu(native_lib):
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    x, w = torch.zeros(2, 4), torch.zeros(6, 4)
+    with pytest.raises(GddimError):
+        ops.gated_ffn(x, w, w, w.t())
+    with pytest.raises(GddimError):
+        ops.gated_ffn_backward(x, x, w, w, w.t(), (x, x, x))
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+def test_float64_block_against_autograd(kind):
+    g = torch.Generator().manual_seed(1)
+    n = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)
+    x, wg, wu, wd, dy = n(5, 6), n(7, 6), n(7, 6), n(4, 7), n(5, 4)
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    f = torch.nn.functional
+    a = f.linear(leaves[0], leaves[1])
+    a = f.silu(a) if kind == "silu" else f.gelu(a, approximate="tanh" if kind == "gelu_tanh" else "none")
+    y = f.linear(a * f.linear(leaves[0], leaves[2]), leaves[3])
+    grads = torch.autograd.grad(y, leaves, dy)
+    got = ref.gated_ffn(x, wg, wu, wd, kind, torch.float64, dy)
+    for a, b in zip(got, (y,) + grads):
+        assert (a.val - b).abs().max() < 1e-12

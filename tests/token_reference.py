@@ -86,3 +86,72 @@ def norm_rotary_backward(dy, x, w, phi, sections, paired, eps):
     dx_mag = rho * (gmag * wv.abs() + xh.abs() * (gmag * wv.abs() * xh.abs()).mean(-1, keepdim=True))
     # rotation, rho twice more than once (its square in the mean's factor): 3 (D + 1)/2 + 12, the mean's own sum D + 1, products 6
     return dx, dx_mag, (g * xh).sum((0, 1, 2)), (gmag * xh.abs()).sum((0, 1, 2)), ROTATION + 3 * (D + 1) / 2 + 12 + D + 1 + 6
+
+
+# ---- gated feed-forward block: values with error bounds carried through the block's own roundings ----
+class V:
+    """A float64 value and a bound on how far the kernel's may be from it."""
+
+    def __init__(self, val, err=None):
+        self.val, self.err = val, torch.zeros_like(val) if err is None else err
+
+    def rounded(self, dtype):
+        """rounded to the tensors' type: half a step, or half the subnormal one"""
+        tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        return V(self.val, self.err + (self.val.abs() + self.err) * half_step(dtype) + tiny)
+
+    def top(self):
+        return self.val.abs() + self.err
+
+    def __mul__(self, o):  # one float32 product
+        return V(self.val * o.val, self.err * o.top() + self.val.abs() * o.err + self.top() * o.top() * U)
+
+    def t(self):
+        return V(self.val.t(), self.err.t())
+
+
+def product(a, b):
+    """a b^T summed in float32 in any order: K products and additions, each term rounded at most K + 1 times, twice that for what the matrix
+    core keeps of the smaller addend"""
+    K = a.val.shape[1]
+    val = a.val @ b.val.t()
+    err = a.err @ b.top().t() + a.val.abs() @ b.err.t() + (2 * (K + 1) * U) * (a.top() @ b.top().t())
+    return V(val, err)
+
+
+def plus(a, b):
+    return V(a.val + b.val, a.err + b.err + (a.top() + b.top()) * U)
+
+
+def act(z, kind):
+    """(activation, derivative) of V z; |act'| < 1.13, |act''| < 0.81; the float32 evaluation loses a few roundings of z, and of (1 + |z|)^3 in the
+    tanh form's polynomial factor"""
+    x = z.val
+    if kind == "silu":
+        s = torch.sigmoid(x)
+        a, d = x * s, s * (1 + x * (1 - s))
+    elif kind == "gelu":
+        c = 0.5 * (1 + torch.erf(x * math.sqrt(0.5)))
+        a, d = x * c, c + x * torch.exp(-0.5 * x * x) / math.sqrt(2 * math.pi)
+    else:
+        k, c = math.sqrt(2 / math.pi), 0.044715
+        t = torch.tanh(k * (x + c * x ** 3))
+        a, d = 0.5 * x * (1 + t), 0.5 * (1 + t) + 0.5 * x * (1 - t * t) * k * (1 + 3 * c * x * x)
+    return V(a, 1.13 * z.err + 16 * U * x.abs()), V(d, 0.81 * z.err + 16 * U * (1 + x.abs()) ** 3)
+
+
+def gated_ffn(x, wg, wu, wd, kind, dtype, dy=None):
+    """y, or (y, dx, dwg, dwu, dwd), as V of their final rounding; gate, up, hidden, dgate and dup are rounded to `dtype` where the block rounds them"""
+    x, wg, wu, wd = (V(t.double()) for t in (x, wg, wu, wd))
+    gate, up = product(x, wg), product(x, wu)
+    hidden = (act(gate, kind)[0] * up).rounded(dtype)
+    y = product(hidden, wd).rounded(dtype)
+    if dy is None:
+        return y
+    dy = V(dy.double())
+    dh = product(dy, wd.t())
+    gate, up = gate.rounded(dtype), up.rounded(dtype)
+    a, d = act(gate, kind)
+    dgate, dup = (dh * up * d).rounded(dtype), (dh * a).rounded(dtype)
+    dx = plus(product(dgate, wg.t()), product(dup, wu.t())).rounded(dtype)
+    return y, dx, product(dgate.t(), x.t()).rounded(dtype), product(dup.t(), x.t()).rounded(dtype), product(dy.t(), hidden.t()).rounded(dtype)
