@@ -15,10 +15,11 @@
 // A fragment is 16 bytes a lane either way: row (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing
 // LDS read gathers it where k is not adjacent), one v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care
 // which k a lane holds as long as both operands agree, so both layouts and all types share one loop.
-// The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m, and stores them with one 8 / 16-byte store.
+// The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m.
 //
-// All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type: gate, up, h (the operands of the next product must be, on the 16-bit
-// matrix core, and gate / up are what a training step keeps), dgate, dup, and the results.
+// All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type are only operands of a next product, as the 16-bit matrix core
+// wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients at
+// 1.8 times the error of one final rounding (relative 3.1e-3 instead of 2.4e-3; 1.7e-3 is the final rounding alone).
 #pragma once
 #include "../common.h"
 #include "../token_ops.h"
@@ -36,24 +37,29 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <typename T> struct quad { typedef T type __attribute__((ext_vector_type(4))); };
 
 // ---- activation and its derivative, float32 ----
-__device__ __forceinline__ float act_value(float z, int act) {
-    if (act == GD_ACT_SILU) return z / (1.f + expf(-z));
-    if (act == GD_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-    return 0.5f * z * (1.f + t);
+// Exponentials and quotients are the hardware's (v_exp_f32, v_rcp_f32, one step of float32 each): an absolute error of a few 2^-24 in a sigmoid or a
+// tanh is the same in its product with z, relative to |z|; with the library's forms the epilogue took as long as the products.
+__device__ __forceinline__ float fast_exp(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504088896341f); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-z)); }
+__device__ __forceinline__ float fast_tanh(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp(2.f * z)); }
+
+template <int ACT> __device__ __forceinline__ float act_value(float z) {
+    if constexpr (ACT == GD_ACT_SILU) return z * sigmoid(z);
+    else if constexpr (ACT == GD_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    else return 0.5f * z * (1.f + fast_tanh(0.79788456080286536f * (z + 0.044715f * z * z * z)));
 }
 
-__device__ __forceinline__ void act_grad(float z, int act, float &a, float &da) {
-    if (act == GD_ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-z));
+template <int ACT> __device__ __forceinline__ void act_grad(float z, float &a, float &da) {
+    if constexpr (ACT == GD_ACT_SILU) {
+        const float s = sigmoid(z);
         a = z * s;
-        da = s * (1.f + z * (1.f - s));
-    } else if (act == GD_ACT_GELU) {
+        da = s + a * (1.f - s);
+    } else if constexpr (ACT == GD_ACT_GELU) {
         const float c = 0.5f * (1.f + erff(z * 0.70710678118654752f));
         a = z * c;
-        da = c + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        da = c + z * 0.39894228040143268f * fast_exp(-0.5f * z * z);
     } else {
-        const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
+        const float t = fast_tanh(0.79788456080286536f * (z + 0.044715f * z * z * z));
         a = 0.5f * z * (1.f + t);
         da = 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
     }
@@ -75,35 +81,53 @@ template <typename T> __device__ __forceinline__ f32x4 load4(const void *p, long
     return v;
 }
 
-// c0 (and c1: up, for EPI_GATED) of row m, columns n .. n + 3
-template <typename T, int EPI>
-__device__ __forceinline__ void epilogue4(const GemmProblem &q, int act, int m, int n, f32x4 c0, f32x4 c1) {
+// row m, columns n .. n + 3; c1: up (EPI_GATED), g / u: gate and up as kept (EPI_GATED_BWD)
+template <typename T, int EPI, int ACT>
+__device__ __forceinline__ void epilogue_act(const GemmProblem &q, int m, int n, f32x4 c0, f32x4 c1, f32x4 g, f32x4 u) {
     const int left = q.N - n;
+    if (m >= q.M || left <= 0) return;
     const bool whole = q.quads && left >= 4;
     const long long o = (long long)m * q.N + n;
     if constexpr (EPI == EPI_STORE) store4<T>(q.out[0], o, c0, left, whole);
     else if constexpr (EPI == EPI_GATED) {
         f32x4 h;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = act_value(c0[i], act) * c1[i];
+        for (int e = 0; e < 4; ++e) h[e] = act_value<ACT>(c0[e]) * c1[e];
         store4<T>(q.out[0], o, h, left, whole);
         if (q.out[1]) {
-            store4<T>(q.out[1], o, c0, left, whole);
-            store4<T>(q.out[2], o, c1, left, whole);
+            store4<float>(q.out[1], o, c0, left, whole);
+            store4<float>(q.out[2], o, c1, left, whole);
         }
     } else {
-        const f32x4 gate = load4<T>(q.in[0], o, left, whole), up = load4<T>(q.in[1], o, left, whole);
         f32x4 dg, du;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int e = 0; e < 4; ++e) {
             float a, da;
-            act_grad(gate[i], act, a, da);
-            dg[i] = c0[i] * up[i] * da;
-            du[i] = c0[i] * a;
+            act_grad<ACT>(g[e], a, da);
+            dg[e] = c0[e] * u[e] * da;
+            du[e] = c0[e] * a;
         }
         store4<T>(q.out[0], o, dg, left, whole);
         store4<T>(q.out[1], o, du, left, whole);
     }
+}
+
+template <typename T, int EPI>
+__device__ __forceinline__ void epilogue(const GemmProblem &q, int act, int m, int n, f32x4 c0, f32x4 c1, f32x4 g, f32x4 u) {
+    if (EPI == EPI_STORE || act == GD_ACT_SILU) epilogue_act<T, EPI, GD_ACT_SILU>(q, m, n, c0, c1, g, u);
+    else if (act == GD_ACT_GELU) epilogue_act<T, EPI, GD_ACT_GELU>(q, m, n, c0, c1, g, u);
+    else epilogue_act<T, EPI, GD_ACT_GELU_TANH>(q, m, n, c0, c1, g, u);
+}
+
+// what EPI_GATED_BWD reads
+__device__ __forceinline__ void load_kept(const GemmProblem &q, int m, int n, f32x4 &g, f32x4 &u) {
+    const int left = q.N - n;
+    g = u = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (m >= q.M || left <= 0) return;
+    const bool whole = q.quads && left >= 4;
+    const long long o = (long long)m * q.N + n;
+    g = load4<float>(q.in[0], o, left, whole);
+    u = load4<float>(q.in[1], o, left, whole);
 }
 
 // ---- one 16-byte fragment each: acc += B-fragment x A-fragment ----
@@ -268,7 +292,8 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p
     constexpr int THREADS = WM * WN * 64;
     constexpr bool GATED = EPI == EPI_GATED;
     constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-    static_assert(!GATED || TN == 64, "a wave's columns are 32 of gate and 32 of up");
+    static_assert(TN == 64 && TM % 64 == 0, "a wave's 64 columns (32 of gate and 32 of up) and groups of 64 rows go through 16 KB of LDS");
+    static_assert(WM * WN * 16384 <= 2 * (BM + BN) * 128, "");
     typedef Operand<T, BM, AKC, THREADS, false> OpA;
     typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
     constexpr int STAGE = OpA::BYTES + OpB::BYTES;
@@ -348,25 +373,62 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p
         if (kt + 1 < kt1) commit(nxt);
     }
 
-    // row m of fragment column j, columns n .. n + 3 of fragment row i
     constexpr int NI = GATED ? FN / 2 : FN;
-    const int mr = m0 + wm * TM + (lane & 15);
-    const int nr = n0 + wn * (GATED ? TN / 2 : TN) + (lane >> 4) * 4;
+    const int mw = m0 + wm * TM, nw = n0 + wn * (GATED ? TN / 2 : TN);  // the wave's first row and column
+    if (q.splits == 1) {
+        // The accumulators go through LDS, 64 rows of the wave at a time (16 KB a wave, 16-byte pieces of row r at piece ^ r), and come back row by row:
+        // global memory is read and written in whole lines, and the loop over them stays a loop (unrolled over the accumulators, three activations
+        // kept the accumulators in scratch memory: dh of 16384 x 4096 x 1024 with its epilogue took 977 us, now 329).
+        constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR, ITER = 64 / RPI, BATCH = 4;
+        char *mine = lds + wave * 16384;
+        __syncthreads();  // every wave has read the last stage
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const int m = mr + j * 16;
-        if (m >= q.M) continue;
+        for (int jc = 0; jc < FM; jc += 4) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int n = nr + i * 16;
-            if (n >= q.N) continue;
-            const f32x4 c1 = GATED ? acc[(i + NI) % FN][j] : f32x4{0.f, 0.f, 0.f, 0.f};
-            if (q.splits == 1) epilogue4<T, EPI>(q, p.act, m, n, acc[i][j], c1);
-            else {  // partial sums, rows padded to whole quads: [split][plane][M][N4]
-                const long long n4 = (q.N + 3) & ~3, plane = (long long)q.M * n4;
-                float *d = q.partial + (long long)w.split * (GATED ? 2 : 1) * plane + (long long)m * n4 + n;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    const int r = j * 16 + (lane & 15);
+                    *reinterpret_cast<f32x4 *>(mine + r * 256 + (((i * 4 + (lane >> 4)) ^ (r & 15)) << 4)) = acc[i][jc + j];
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int piece = lane & (LPR - 1), n = nw + piece * 4;
+#pragma unroll 1
+            for (int it = 0; it < ITER; it += BATCH) {
+                f32x4 g[BATCH], u[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    g[k] = u[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if constexpr (EPI == EPI_GATED_BWD) load_kept(q, mw + jc * 16 + (it + k) * RPI + lane / LPR, n, g[k], u[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int r = (it + k) * RPI + lane / LPR;
+                    const f32x4 c0 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + ((piece ^ (r & 15)) << 4));
+                    f32x4 c1 = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (GATED) c1 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + (((piece + 8) ^ (r & 15)) << 4));
+                    epilogue<T, EPI>(q, p.act, mw + jc * 16 + r, n, c0, c1, g[k], u[k]);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    } else {
+        // partial sums, rows padded to whole quads: [split][plane][M][N4]
+        const long long n4 = (q.N + 3) & ~3, plane = (long long)q.M * n4;
+        float *part = q.partial + (long long)w.split * (GATED ? 2 : 1) * plane;
+        const int nr = nw + (lane >> 4) * 4;
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            const int m = mw + (lane & 15) + j * 16;
+            if (m >= q.M) continue;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                if (nr + i * 16 >= q.N) continue;
+                float *d = part + (long long)m * n4 + nr + i * 16;
                 *reinterpret_cast<f32x4 *>(d) = acc[i][j];
-                if constexpr (GATED) *reinterpret_cast<f32x4 *>(d + plane) = c1;
+                if constexpr (GATED) *reinterpret_cast<f32x4 *>(d + plane) = acc[(i + NI) % FN][j];
             }
         }
     }
@@ -391,7 +453,9 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmLaunch p) {
         c0 += *reinterpret_cast<const f32x4 *>(d + (long long)s * (GATED ? 2 : 1) * plane);
         if constexpr (GATED) c1 += *reinterpret_cast<const f32x4 *>(d + (long long)s * 2 * plane + plane);
     }
-    epilogue4<T, EPI>(q, p.act, m, n, c0, c1);
+    f32x4 g = {0.f, 0.f, 0.f, 0.f}, u = g;
+    if constexpr (EPI == EPI_GATED_BWD) load_kept(q, m, n, g, u);
+    epilogue<T, EPI>(q, p.act, m, n, c0, c1, g, u);
 }
 
 template <typename T, bool AKC, bool BKC, int EPI>

@@ -130,7 +130,7 @@ int run_gemm(GemmLaunch &l, int dtype, GemmKind kind, float *partial, hipStream_
         GemmProblem &q = l.q[i];
         q.quads = q.N % 4 == 0;
         for (const void *o : {(const void *)q.out[0], (const void *)q.out[1], (const void *)q.out[2], q.in[0], q.in[1]})
-            if ((uintptr_t)o % (4 * elem_size(dtype))) q.quads = 0;
+            if ((uintptr_t)o % 16) q.quads = 0;
         q.partial = partial;
         if (q.splits > 1) partial += (long long)q.splits * (gated ? 2 : 1) * q.M * ((q.N + 3LL) / 4 * 4);
         blocks += q.blocks;
@@ -195,7 +195,7 @@ long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward) {
     return 2 * grad + partial_floats(f, d->dtype, GEMM_DHIDDEN, GEMM_DW) * (long long)sizeof(float);
 }
 
-int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, void *gate_dev, void *up_dev,
+int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, float *gate_dev, float *up_dev,
                  void *hidden_dev, void *y, void *workspace_dev, void *stream) {
     static const char *who = "gated_ffn";
     GD_TRY(check_ffn(d, who));
@@ -214,7 +214,7 @@ int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const 
 }
 
 int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy, const void *x, const void *w_gate, const void *w_up,
-                          const void *w_down, const void *gate, const void *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
+                          const void *w_down, const float *gate, const float *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
                           void *dw_down, void *workspace_dev, void *stream) {
     static const char *who = "gated_ffn_backward";
     GD_TRY(check_ffn(d, who));

@@ -54,8 +54,8 @@ struct GemmProblem {
     long long lda, ldb;          // bytes from row to row of the matrix as it lies in memory
     long long a_bytes, b_bytes;  // extent of a matrix in memory
     int M, N, K, parts;
-    void *out[3];                // rows of N elements, dense
-    const void *in[2];           // EPI_GATED_BWD: gate, up
+    void *out[3];                // rows of N elements, dense; EPI_GATED: h, gate and up (float32 or null); EPI_GATED_BWD: dgate, dup
+    const void *in[2];           // EPI_GATED_BWD: gate, up (float32)
     int quads;                   // N % 4 == 0 and outputs aligned: four columns per store
     int splits, steps_per_split;
     float *partial;

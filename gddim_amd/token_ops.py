@@ -268,14 +268,14 @@ def _workspace(desc, backward, device):
 def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
     """Gated feed-forward block (act(x w_gate^T) * (x w_up^T)) w_down^T: x (..., in), weights as torch.nn.Linear keeps them -- w_gate and w_up
     (hidden, in), w_down (out, hidden) -- act 'silu', 'gelu' or 'gelu_tanh'.  Returns y (..., out); with save=True (y, saved), saved for
-    gated_ffn_backward.  Both projections, the activation and the product are one kernel."""
+    gated_ffn_backward (the two projections in float32 and their product).  Both projections, the activation and the product are one kernel."""
     torch = _torch()[0]
     shape = x.shape[:-1] if isinstance(x, torch.Tensor) else ()
     x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
     M, F = x.shape[0], w_gate.shape[0]
     y = torch.empty((M, w_down.shape[0]), dtype=x.dtype, device=x.device)
     hidden = torch.empty((M, F), dtype=x.dtype, device=x.device)
-    gate, up = (torch.empty_like(hidden), torch.empty_like(hidden)) if save else (None, None)
+    gate, up = (torch.empty((M, F), dtype=torch.float32, device=x.device) for _ in range(2)) if save else (None, None)
     with _Device(x) as stream:
         ws = _workspace(desc, 0, x.device)
         check(_abi.lib().gd_gated_ffn(desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
@@ -297,7 +297,9 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
     if not isinstance(saved, tuple) or len(saved) != 3:
         raise GddimError("saved: expected the second result of gated_ffn(..., save=True)")
     for t, name in zip(saved, ("gate", "up", "hidden")):
-        _like(t, "saved " + name, x, "x")
+        _on_gpu(t, "saved " + name)
+        if t.dtype != (x.dtype if name == "hidden" else torch.float32) or t.device != x.device:
+            raise GddimError("saved %s is %s on %s: not what gated_ffn(..., save=True) gave for x" % (name, t.dtype, t.device))
         if tuple(t.shape) != (M, F) or not t.is_contiguous():
             raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
     dy = _rows(dy, O)

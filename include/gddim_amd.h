@@ -400,15 +400,15 @@ typedef struct gd_ffn_desc {
     int rows, in, hidden, out;
     long long ld_x, ld_w_in, ld_w_down;
 } gd_ffn_desc;
-/* hidden_dev (rows, hidden) receives act(gate) (.) up; gate_dev and up_dev (rows, hidden) the projections, or both null: what the backward call
- * needs of a training step.  workspace_dev: gd_gated_ffn_workspace(d, 0) bytes (may be 0), 16-byte aligned. */
+/* hidden_dev (rows, hidden) receives act(gate) (.) up; gate_dev and up_dev (rows, hidden) the projections in fp32 whatever the tensors' type, or both
+ * null: what the backward call needs of a training step.  workspace_dev: gd_gated_ffn_workspace(d, 0) bytes (may be 0), 16-byte aligned. */
 long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward);
-int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, void *gate_dev, void *up_dev,
+int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, float *gate_dev, float *up_dev,
                  void *hidden_dev, void *y, void *workspace_dev, void *stream);
 /* Gradients from dy (rows, out; rows ld_dy apart) and what the forward call kept: dx (rows, in), dw_gate, dw_up (hidden, in), dw_down (out, hidden), all
  * dense.  workspace_dev: gd_gated_ffn_workspace(d, 1) bytes, 16-byte aligned.  The same bits every time. */
 int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy, const void *x, const void *w_gate, const void *w_up,
-                          const void *w_down, const void *gate, const void *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
+                          const void *w_down, const float *gate, const float *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
                           void *dw_down, void *workspace_dev, void *stream);
 
 #ifdef __cplusplus

@@ -141,7 +141,7 @@ def act(z, kind):
 
 
 def gated_ffn(x, wg, wu, wd, kind, dtype, dy=None):
-    """y, or (y, dx, dwg, dwu, dwd), as V of their final rounding; gate, up, hidden, dgate and dup are rounded to `dtype` where the block rounds them"""
+    """y, or (y, dx, dwg, dwu, dwd), as V of their final rounding; hidden, dgate and dup are rounded to `dtype` where the block rounds them"""
     x, wg, wu, wd = (V(t.double()) for t in (x, wg, wu, wd))
     gate, up = product(x, wg), product(x, wu)
     hidden = (act(gate, kind)[0] * up).rounded(dtype)
@@ -150,7 +150,6 @@ def gated_ffn(x, wg, wu, wd, kind, dtype, dy=None):
         return y
     dy = V(dy.double())
     dh = product(dy, wd.t())
-    gate, up = gate.rounded(dtype), up.rounded(dtype)
     a, d = act(gate, kind)
     dgate, dup = (dh * up * d).rounded(dtype), (dh * a).rounded(dtype)
     dx = plus(product(dgate, wg.t()), product(dup, wu.t())).rounded(dtype)
