@@ -9,13 +9,17 @@
 // C[m][n] = sum_k A[m][k] B[n][k].  Each operand lies in memory with k adjacent (KC: x, weights as torch.nn.Linear keeps them) or with its other index
 // adjacent (the weights in dh and dx, everything in the weights' gradients); no operand is transposed in memory.
 //
-// Tiles.  A step of the k loop stages 128 bytes of k (64 16-bit or 32 float32 values) for BM rows of A and BN of B in LDS, two stages.  KC rows are 128 bytes =
-// 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  Global memory goes to LDS directly, 16 bytes a
-// lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole 16-byte pieces, through registers.
-// A fragment is 16 bytes a lane either way: row (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing
-// LDS read gathers it where k is not adjacent), one v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care
-// which k a lane holds as long as both operands agree, so both layouts and all types share one loop.
-// The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m.
+// Tiles.  A step of the k loop takes 64 bytes of k (32 16-bit or 16 float32 values) of BM rows of A and BN of B.  A fragment is 16 bytes a lane: row
+// (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing LDS read gathers it where k is not adjacent), one
+// v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care which k a lane holds as long as both operands agree, so
+// both layouts and all types share one loop.  The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m.
+// Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole
+// 16-byte pieces, through registers.  KC rows take whole 128-byte lines, two steps a stage, 8 pieces of 16, piece c of row r at c ^ swizzle(r): with
+// 64-byte rows the requests to L2 doubled and became the bound (y of 16384 x 1024 x 4096: 153 us instead of 129).  Other operands keep their k rows, pieces
+// moved by k.  No bank conflicts either way (counted).
+// Step k multiplies fragments that were read during step k - 1, while those of step k + 1 are read.  Stages lie in a ring: two of two steps, or four of one
+// step where no operand is KC; a stage is requested into the place of one that all waves have read, two / three steps (2048 / 3072 MFMA cycles of a
+// 256 x 256 tile) before it is read.
 //
 // All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type are only operands of a next product, as the 16-bit matrix core
 // wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients at
@@ -147,16 +151,34 @@ template <> __device__ __forceinline__ f32x4 mma<float>(i32x4 b, i32x4 a, f32x4 
 
 __device__ __forceinline__ int kc_swizzle(int row) { return (row >> 1) & 7; }
 
+// a raw buffer of `bytes` bytes: reads past its end give zeros
+__device__ __forceinline__ i32x4 buffer_of(const char *p, int bytes) {
+    const unsigned long long v = (unsigned long long)p;
+    i32x4 r = {(int)(unsigned)v, (int)((unsigned)(v >> 32) & 0xffffu), bytes, 0x00020000};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    return r;
+}
+
+// 16 bytes a lane from buffer + off straight to LDS at lds + 16 lane.  Written out rather than taken from the builtin, after which the compiler
+// waits for every such request (vmcnt(0)) before each transposing LDS read, though the ring keeps their places apart: wait_loads + lds_barrier below say when
+// a stage has arrived.  The instruction has no register result.
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned off, char *lds) {
+    const int at = __builtin_amdgcn_readfirstlane((int)(unsigned long long)(__attribute__((address_space(3))) char *)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(buffer) : "memory", "m0");
+}
+
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;  // a buffer offset past every num_records used here: the piece arrives as zeros
 
-// One operand: R rows (of m or n) x 128 bytes of k per stage
-template <typename T, int R, bool KC, int THREADS, bool GATED_B>
+// One operand: R rows (of m or n) x STEPS * 64 bytes of k per stage
+template <typename T, int R, bool KC, int STEPS, int THREADS, bool GATED_B>
 struct Operand {
-    static constexpr int ES = sizeof(T), KSTEP = 128 / ES, V = 16 / ES;   // k per stage, elements of a piece
+    static_assert(!KC || STEPS == 2, "rows of whole 128-byte lines");
+    static constexpr int ES = sizeof(T), KSTAGE = STEPS * 64 / ES, V = 16 / ES;  // k per stage, elements of a piece
     static constexpr int WAVES = THREADS / 64;
-    static constexpr int PIECES = R * 8 / THREADS;                        // 16-byte pieces a thread stages
+    static constexpr int PIECES = R * 4 * STEPS / THREADS;                // 16-byte pieces a thread stages
     static constexpr int CPR = KC ? 8 : R * ES / 16;                      // pieces of an LDS row
-    static constexpr int BYTES = R * 128;
+    static constexpr int BYTES = R * 64 * STEPS;
 
     const char *base[2];   // element (first row, k = 0) of each source
     long long end[2];      // bytes from there to the end of the matrix
@@ -182,17 +204,16 @@ struct Operand {
     __device__ static __forceinline__ int source_of(int r) { return GATED_B ? (r >> 5) & 1 : 0; }
     __device__ static __forceinline__ int row_in_source(int r) { return GATED_B ? ((r >> 6) << 5) + (r & 31) : r; }
 
-    // stage the 128 bytes of k from step kt (src: which source of a two-part sum) straight into LDS
-    __device__ __forceinline__ void stage_direct(char *lds, int src, int kt, int wave) const {
-#ifdef __HIP_DEVICE_COMPILE__  // the host pass has no buffer descriptors
-        const long long adv = KC ? (long long)kt * 128 : (long long)kt * KSTEP * ld;
-        __amdgpu_buffer_rsrc_t rs[GATED_B ? 2 : 1];
+    // stage st (src: which source of a two-part sum) straight into LDS
+    __device__ __forceinline__ void stage_direct(char *lds, int src, int st, int wave) const {
+        const long long adv = KC ? (long long)st * 128 : (long long)st * KSTAGE * ld;
+        i32x4 rs[GATED_B ? 2 : 1];
 #pragma unroll
         for (int g = 0; g < (GATED_B ? 2 : 1); ++g) {
             const int s = GATED_B ? g : src;
             long long left = end[s] - adv;
             left = left < 0 ? 0 : left > 0x7fffffffLL ? 0x7fffffffLL : left;
-            rs[g] = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base[s]) + adv, 0, (int)left, 0x00020000);
+            rs[g] = buffer_of(base[s] + adv, (int)left);
         }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -200,22 +221,21 @@ struct Operand {
             bool in;
             if constexpr (KC) {
                 off = (unsigned)row_in_source(row[i]) * (unsigned)ld + piece[i] * 16;
-                in = kt * KSTEP + piece[i] * V < k_len;
+                in = st * KSTAGE + piece[i] * V < k_len;
             } else {
                 off = (unsigned)row[i] * (unsigned)ld + piece[i] * 16;
-                in = kt * KSTEP + row[i] < k_len;
+                in = st * KSTAGE + row[i] < k_len;
             }
             off = in ? off : OUT_OF_RANGE;
             const int g = GATED_B ? source_of((i * WAVES + wave) * 64 / CPR) : 0;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs[g], (__attribute__((address_space(3))) void *)(lds + (i * WAVES + wave) * 1024), 16, off, 0, 0, 0);
+            load_to_lds(rs[g], off, lds + (i * WAVES + wave) * 1024);
         }
-#endif
     }
     // ... through registers, for rows that are not whole aligned pieces
-    __device__ __forceinline__ void load_regs(i32x4 *r, int src, int kt) const {
+    __device__ __forceinline__ void load_regs(i32x4 *r, int src, int st) const {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int k0 = kt * KSTEP + (KC ? piece[i] * V : row[i]);
+            const int k0 = st * KSTAGE + (KC ? piece[i] * V : row[i]);
             const int s = GATED_B ? source_of(row[i]) : src;
             const int rr = KC ? row_in_source(row[i]) : piece[i] * V;  // first row / column
             const char *p = KC ? base[s] + (long long)rr * ld + (long long)k0 * ES : base[s] + (long long)k0 * ld + (long long)rr * ES;
@@ -236,32 +256,43 @@ struct Operand {
         for (int i = 0; i < PIECES; ++i) *reinterpret_cast<i32x4 *>(lds + ((i * WAVES + wave) * 64 + lane) * 16) = r[i];
     }
 
-    // fragment: rows r0 + lane % 16, half kk of the stage's k
-    __device__ static __forceinline__ i32x4 fragment(const char *lds, int r0, int kk, int lane) {
+    // fragment: rows r0 + lane % 16, k of the stage's step `sub`
+    __device__ static __forceinline__ i32x4 fragment(const char *lds, int r0, int sub, int lane) {
         const int i = lane & 15, g = lane >> 4;
         if constexpr (KC) {
             const int r = r0 + i;
-            return *reinterpret_cast<const i32x4 *>(lds + r * 128 + (((kk * 4 + g) ^ kc_swizzle(r)) << 4));
+            return *reinterpret_cast<const i32x4 *>(lds + r * 128 + (((sub * 4 + g) ^ kc_swizzle(r)) << 4));
         } else if constexpr (ES == 2) {
             typedef __attribute__((address_space(3))) i16x4 *lds_ptr;
-            i16x8 v;
-            const int k = kk * 32 + g * 8 + (i >> 2);
+            const int k = sub * 32 + g * 8 + (i >> 2);
             const char *p = lds + k * (R * 2) + (((r0 / 8 + ((i & 3) >> 1)) ^ swizzle(k)) << 4) + (i & 1) * 8;
             const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
             const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * R * 2));
-            v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            return __builtin_bit_cast(i32x4, v);
+            return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             f32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int k = (kk * 4 + g) * 4 + j, c = r0 + i;
+                const int k = sub * 16 + g * 4 + j, c = r0 + i;
                 v[j] = *reinterpret_cast<const float *>(lds + k * (R * 4) + (((c >> 2) ^ swizzle(k)) << 4) + (c & 3) * 4);
             }
             return __builtin_bit_cast(i32x4, v);
         }
     }
 };
+
+// s_waitcnt vmcnt(n), the other counters left alone
+template <int N> __device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+// what this wave wrote to and read from LDS is done, and so it is for everyone; requests to global memory stay on their way
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // workgroup -> (problem, tile, split): workgroups go round-robin over the 8 XCDs, each with an L2 of its own; consecutive tiles of one XCD share
 // operand rows, eight m tiles to a group
@@ -293,12 +324,13 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p
     constexpr bool GATED = EPI == EPI_GATED;
     constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     static_assert(TN == 64 && TM % 64 == 0, "a wave's 64 columns (32 of gate and 32 of up) and groups of 64 rows go through 16 KB of LDS");
-    static_assert(WM * WN * 16384 <= 2 * (BM + BN) * 128, "");
-    typedef Operand<T, BM, AKC, THREADS, false> OpA;
-    typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
-    constexpr int STAGE = OpA::BYTES + OpB::BYTES;
-    constexpr int KSTEP = OpA::KSTEP;
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+    constexpr int STEPS = AKC || BKC || !DIRECT ? 2 : 1, RING = 4 / STEPS;
+    typedef Operand<T, BM, AKC, STEPS, THREADS, false> OpA;
+    typedef Operand<T, BN, BKC, STEPS, THREADS, GATED> OpB;
+    constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES;
+    static_assert(WM * WN * 16384 <= RING * STAGE, "");
+    constexpr int KSTAGE = OpA::KSTAGE;
+    __shared__ __attribute__((aligned(16))) char lds[RING * STAGE];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -323,9 +355,9 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p
         a.end[s] = q.a_bytes - oa;
         b.end[s] = q.b_bytes - ob;
     }
-    const int per_part = (q.K + KSTEP - 1) / KSTEP;       // steps of one part of the sum
-    const int kt0 = w.split * q.steps_per_split;
-    const int kt1 = min(kt0 + q.steps_per_split, per_part * q.parts);
+    const int per_part = (q.K + KSTAGE - 1) / KSTAGE;  // stages of one part of the sum
+    const int st0 = w.split * q.stages_per_split;
+    const int st1 = min(st0 + q.stages_per_split, per_part * q.parts);
 
     f32x4 acc[FN][FM];
 #pragma unroll
@@ -334,43 +366,90 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     i32x4 ra[DIRECT ? 1 : OpA::PIECES], rb[DIRECT ? 1 : OpB::PIECES];
-    auto fetch = [&](int kt, char *stage) __attribute__((always_inline)) {
-        const int src = kt >= per_part, k = src ? kt - per_part : kt;
+    auto place_of = [&](int st) __attribute__((always_inline)) { return lds + ((st - st0) & (RING - 1)) * STAGE; };
+    auto fetch = [&](int st) __attribute__((always_inline)) {
+        const int src = st >= per_part, k = src ? st - per_part : st;
         if constexpr (DIRECT) {
-            a.stage_direct(stage, src, k, wave);
-            b.stage_direct(stage + OpA::BYTES, src, k, wave);
+            a.stage_direct(place_of(st), src, k, wave);
+            b.stage_direct(place_of(st) + OpA::BYTES, src, k, wave);
         } else {
             a.load_regs(ra, src, k);
             b.load_regs(rb, src, k);
         }
     };
-    auto commit = [&](char *stage) __attribute__((always_inline)) {
-        if constexpr (!DIRECT) {
-            a.store_regs(stage, ra, wave, lane);
-            b.store_regs(stage + OpA::BYTES, rb, wave, lane);
+    auto commit = [&](int st) __attribute__((always_inline)) {
+        a.store_regs(place_of(st), ra, wave, lane);
+        b.store_regs(place_of(st) + OpA::BYTES, rb, wave, lane);
+    };
+    i32x4 fa[2][FM], fb[2][FN];
+    auto read = [&](int st, int sub, int set) __attribute__((always_inline)) {
+        const char *at = place_of(st);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fb[set][i] = OpB::fragment(at + OpA::BYTES, wn * TN + i * 16, sub, lane);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) fa[set][j] = OpA::fragment(at, wm * TM + j * 16, sub, lane);
+    };
+    auto multiply = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = mma<T>(fb[set][i], fa[set][j], acc[i][j]);
+    };
+    // step `sub` of stage st, its fragments in (or on their way to) set.  At the stage's last step all its fragments have been read: behind the barrier its place
+    // is free and the next stage complete.  full: stages up to st + RING exist (no conditions in the long part of the loop)
+    auto step = [&](int st, int sub, int set, bool full) __attribute__((always_inline)) {
+        if (sub + 1 < STEPS) read(st, sub + 1, set ^ 1);
+        else if (full || st + 1 < st1) {
+            if constexpr (DIRECT) {
+                if (full || st + RING - 1 < st1) wait_loads<(RING - 2) * LOADS>();  // stages up to st + RING - 1 have been requested
+                else wait_loads<0>();
+            } else commit(st + 1);
+            lds_barrier();
+            if constexpr (DIRECT) {
+                if (full || st + RING < st1) fetch(st + RING);
+            } else {
+                if (full || st + 2 < st1) fetch(st + 2);
+            }
+            read(st + 1, 0, set ^ 1);
         }
+        multiply(set);
+        __builtin_amdgcn_sched_barrier(0);  // the products stay between the reads and the next barrier: they cover the reads' way
     };
 
-    fetch(kt0, lds);
-    commit(lds);
-    for (int kt = kt0; kt < kt1; ++kt) {
-        char *cur = lds + ((kt - kt0) & 1) * STAGE, *nxt = lds + ((kt - kt0 + 1) & 1) * STAGE;
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces of the current stage are in LDS ...
-        __syncthreads();                     // ... and everyone's; the other stage has been read by all
-        if (kt + 1 < kt1) fetch(kt + 1, nxt);
+    if (st0 < st1) {
+        if constexpr (DIRECT) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            i32x4 fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FM; ++j) fa[j] = OpA::fragment(cur, wm * TM + j * 16, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FN; ++i) fb[i] = OpB::fragment(cur + OpA::BYTES, wn * TN + i * 16, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = mma<T>(fb[i], fa[j], acc[i][j]);
+            for (int k = 0; k < RING; ++k)
+                if (st0 + k < st1) fetch(st0 + k);
+            if (st0 + RING <= st1) wait_loads<(RING - 1) * LOADS>();
+            else wait_loads<0>();
+        } else {
+            fetch(st0);
+            commit(st0);
+            if (st0 + 1 < st1) fetch(st0 + 1);
         }
-        if (kt + 1 < kt1) commit(nxt);
+        lds_barrier();
+        read(st0, 0, 0);
+        int st = st0;
+        if constexpr (STEPS == 2) {
+            for (; st + RING < st1; ++st) {
+                step(st, 0, 0, true);
+                step(st, 1, 1, true);
+            }
+            for (; st < st1; ++st) {
+                step(st, 0, 0, false);
+                step(st, 1, 1, false);
+            }
+        } else {
+            for (; st + 1 + RING < st1; st += 2) {
+                step(st, 0, 0, true);
+                step(st + 1, 0, 1, true);
+            }
+            for (; st < st1; st += 2) {
+                step(st, 0, 0, false);
+                if (st + 1 < st1) step(st + 1, 0, 1, false);
+            }
+        }
     }
 
     constexpr int NI = GATED ? FN / 2 : FN;

@@ -81,9 +81,10 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
 }
 
 // tile and split of a launch; returns the floats of partial sums it needs, or -1 (more workgroups than a grid holds)
-long long plan_gemm(GemmLaunch &l, int dtype, bool gated) {
+long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
+    const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
-    const int kstep = 128 / (int)elem_size(dtype);
+    const int kstage = (kind == GEMM_DW && l.direct ? 64 : 128) / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
     auto tiles = [&](int t) {
         long long n = 0;
         for (int i = 0; i < l.problems; ++i) n += ((l.q[i].M + t - 1LL) / t) * ((l.q[i].N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
@@ -99,14 +100,14 @@ long long plan_gemm(GemmLaunch &l, int dtype, bool gated) {
         GemmProblem &q = l.q[i];
         q.tiles_m = (int)((q.M + t - 1LL) / t);
         q.tiles_n = (int)((q.N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
-        const long long steps = (long long)q.parts * ((q.K + kstep - 1) / kstep);
-        // few tiles and a long sum: split it over workgroups, at least 4 steps each
+        const long long stages = (long long)q.parts * ((q.K + kstage - 1) / kstage);
+        // few tiles and a long sum: split it over workgroups, at least 4 stages each
         long long splits = all > 0 ? room / all : 1;
-        if (splits > steps / 4) splits = steps / 4;
+        if (splits > stages / 4) splits = stages / 4;
         if (splits > 16) splits = 16;
         if (splits < 1) splits = 1;
-        q.steps_per_split = (int)((steps + splits - 1) / splits);
-        q.splits = q.steps_per_split ? (int)((steps + q.steps_per_split - 1) / q.steps_per_split) : 1;
+        q.stages_per_split = (int)((stages + splits - 1) / splits);
+        q.splits = q.stages_per_split ? (int)((stages + q.stages_per_split - 1) / q.stages_per_split) : 1;
         q.blocks = q.tiles_m * q.tiles_n * q.splits;
         blocks += q.blocks;
         q.join_threads = 0;
@@ -124,7 +125,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, bool gated) {
 
 int run_gemm(GemmLaunch &l, int dtype, GemmKind kind, float *partial, hipStream_t s, const char *who) {
     const bool gated = kind == GEMM_GATE_UP;
-    GD_CHECK(plan_gemm(l, dtype, gated) >= 0, "%s: too many tiles for one launch", who);
+    GD_CHECK(plan_gemm(l, dtype, kind) >= 0, "%s: too many tiles for one launch", who);
     int blocks = 0;
     for (int i = 0; i < l.problems; ++i) {
         GemmProblem &q = l.q[i];
@@ -177,7 +178,7 @@ long long partial_floats(FfnLaunches f, int dtype, int first, int last) {
         for (int direct = 0; direct < 2; ++direct) {
             GemmLaunch l = f.l[k];
             l.direct = direct;
-            const long long n = plan_gemm(l, dtype, k == GEMM_GATE_UP);
+            const long long n = plan_gemm(l, dtype, (GemmKind)k);
             if (n > most) most = n;
         }
     return most;

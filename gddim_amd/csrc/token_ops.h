@@ -57,7 +57,7 @@ struct GemmProblem {
     void *out[3];                // rows of N elements, dense; EPI_GATED: h, gate and up (float32 or null); EPI_GATED_BWD: dgate, dup
     const void *in[2];           // EPI_GATED_BWD: gate, up (float32)
     int quads;                   // N % 4 == 0 and outputs aligned: four columns per store
-    int splits, steps_per_split;
+    int splits, stages_per_split;
     float *partial;
     // filled in by the launcher
     int tiles_m, tiles_n, blocks;
