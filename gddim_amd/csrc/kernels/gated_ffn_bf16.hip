@@ -3,6 +3,6 @@
 
 namespace gd {
 
-int launch_ffn_gemm_bf16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s) { return ffn::launch_type<__bf16>(p, kind, blocks, s); }
+int launch_ffn_gemm_bf16(const GemmLaunch &p, GemmKind kind, hipStream_t s) { return ffn::launch_type<__bf16>(p, kind, s); }
 
 }  // namespace gd

@@ -3,6 +3,6 @@
 
 namespace gd {
 
-int launch_ffn_gemm_f16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s) { return ffn::launch_type<_Float16>(p, kind, blocks, s); }
+int launch_ffn_gemm_f16(const GemmLaunch &p, GemmKind kind, hipStream_t s) { return ffn::launch_type<_Float16>(p, kind, s); }
 
 }  // namespace gd

@@ -13,13 +13,13 @@
 // (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing LDS read gathers it where k is not adjacent), one
 // v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care which k a lane holds as long as both operands agree, so
 // both layouts and all types share one loop.  The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m.
-// Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole
-// 16-byte pieces, through registers.  KC rows take whole 128-byte lines, two steps a stage, 8 pieces of 16, piece c of row r at c ^ swizzle(r): with
-// 64-byte rows the requests to L2 doubled and became the bound (y of 16384 x 1024 x 4096: 153 us instead of 129).  Other operands keep their k rows, pieces
-// moved by k.  No bank conflicts either way (counted).
-// Step k multiplies fragments that were read during step k - 1, while those of step k + 1 are read.  Stages lie in a ring: two of two steps, or four of one
-// step where no operand is KC; a stage is requested into the place of one that all waves have read, two / three steps (2048 / 3072 MFMA cycles of a
-// 256 x 256 tile) before it is read.
+// A stage is two steps, 128 bytes of k: KC rows take whole lines (with 64-byte rows the requests to L2 doubled and became the bound: y of 16384 x 1024 x
+// 4096 in 153 us instead of 129), 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  No bank conflicts
+// either way (counted).  Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows
+// are not whole 16-byte pieces, through registers.
+// Two stages lie in LDS.  A step multiplies fragments that were read during the step before, those of the next are read between its products: when a stage's
+// second step begins all of it has been read, and the stage after the next is requested into its place, two steps (2048 MFMA cycles of a 256 x 256
+// tile) before it is needed.
 //
 // All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type are only operands of a next product, as the 16-bit matrix core
 // wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients at
@@ -32,6 +32,7 @@ namespace gd {
 namespace ffn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
@@ -134,18 +135,21 @@ __device__ __forceinline__ void load_kept(const GemmProblem &q, int m, int n, f3
     u = load4<float>(q.in[1], o, left, whole);
 }
 
+// of a 32 x 32 block in the accumulators, lane l holds row l % 32 and columns 8 e + 4 (l / 32) .. + 3, e = 0 .. 3
+__device__ __forceinline__ f32x4 quad_of(const f32x16 &c, int e) { return f32x4{c[4 * e], c[4 * e + 1], c[4 * e + 2], c[4 * e + 3]}; }
+
 // ---- one 16-byte fragment each: acc += B-fragment x A-fragment ----
-template <typename T> __device__ __forceinline__ f32x4 mma(i32x4 b, i32x4 a, f32x4 c);
-template <> __device__ __forceinline__ f32x4 mma<__bf16>(i32x4 b, i32x4 a, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+template <typename T> __device__ __forceinline__ f32x16 mma(i32x4 b, i32x4 a, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mma<__bf16>(i32x4 b, i32x4 a, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x4 mma<_Float16>(i32x4 b, i32x4 a, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
+template <> __device__ __forceinline__ f32x16 mma<_Float16>(i32x4 b, i32x4 a, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x4 mma<float>(i32x4 b, i32x4 a, f32x4 c) {
+template <> __device__ __forceinline__ f32x16 mma<float>(i32x4 b, i32x4 a, f32x16 c) {
     const f32x4 bf = __builtin_bit_cast(f32x4, b), af = __builtin_bit_cast(f32x4, a);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[i], af[i], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(bf[i], af[i], c, 0, 0, 0);
     return c;
 }
 
@@ -170,74 +174,73 @@ __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned off, char *ld
 
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;  // a buffer offset past every num_records used here: the piece arrives as zeros
 
-// One operand: R rows (of m or n) x STEPS * 64 bytes of k per stage
-template <typename T, int R, bool KC, int STEPS, int THREADS, bool GATED_B>
+// One operand: R rows (of m or n) x 128 bytes of k per stage
+template <typename T, int R, bool KC, int THREADS, bool GATED_B>
 struct Operand {
-    static_assert(!KC || STEPS == 2, "rows of whole 128-byte lines");
-    static constexpr int ES = sizeof(T), KSTAGE = STEPS * 64 / ES, V = 16 / ES;  // k per stage, elements of a piece
+    static constexpr int ES = sizeof(T), KSTAGE = 128 / ES, V = 16 / ES;  // k per stage, elements of a piece
     static constexpr int WAVES = THREADS / 64;
-    static constexpr int PIECES = R * 4 * STEPS / THREADS;                // 16-byte pieces a thread stages
+    static constexpr int PIECES = R * 8 / THREADS;                        // 16-byte pieces a thread stages
     static constexpr int CPR = KC ? 8 : R * ES / 16;                      // pieces of an LDS row
-    static constexpr int BYTES = R * 64 * STEPS;
+    static constexpr int BYTES = R * 128;
+
+    // A piece's slot in the stage: (i * WAVES + wave) * 64 + lane, slot / CPR its row (KC: of the matrix tile; else of k).  Its first row is the same for a wave's 64
+    // slots, and the swizzle of row i repeats every PERIOD i: a lane keeps PERIOD offsets, the rest of an address is the wave's.
+    static constexpr int RPI = 64 / CPR, PERIOD = 1;
+    static_assert(PIECES % PERIOD == 0 && (KC ? WAVES * RPI % 16 == 0 : ES == 2 ? WAVES * RPI % 4 == 0 : WAVES * RPI % 8 == 0), "");
 
     const char *base[2];   // element (first row, k = 0) of each source
-    long long end[2];      // bytes from there to the end of the matrix
+    long long end;         // bytes from there to the end of the matrix
     long long ld;          // bytes
     int k_len;             // k of one source
     int rows_left;         // rows (KC) / columns (else) from the tile's first
-    int row[PIECES], piece[PIECES];  // of the matrix tile: KC row / k row; source piece
 
-    __device__ __forceinline__ void init(int wave, int lane) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int slot = (i * WAVES + wave) * 64 + lane;  // 16-byte slot of the stage
-            row[i] = slot / CPR;
-            piece[i] = (slot % CPR) ^ swizzle(row[i]);
-        }
-    }
+    __device__ static __forceinline__ int row_of(int i, int wave, int lane) { return (i * WAVES + wave) * RPI + lane / CPR; }
+    __device__ static __forceinline__ int piece_of(int i, int wave, int lane) { return lane % CPR ^ swizzle(row_of(i % PERIOD, wave, lane)); }
     __device__ static __forceinline__ int swizzle(int r) {
         if constexpr (KC) return kc_swizzle(r);
-        else if constexpr (ES == 2) return 2 * (r & 3) + 8 * ((r >> 3) & 1);
-        else return 4 * ((r >> 2) & 3);
+        else if constexpr (ES == 2) return 4 * (r & 3);
+        else return 8 * ((r >> 2) & 1);
     }
     // gated B tiles: rows of gate and up alternate in blocks of 32, so that a wave's 64 columns hold both of its 32
     __device__ static __forceinline__ int source_of(int r) { return GATED_B ? (r >> 5) & 1 : 0; }
     __device__ static __forceinline__ int row_in_source(int r) { return GATED_B ? ((r >> 6) << 5) + (r & 31) : r; }
 
-    // stage st (src: which source of a two-part sum) straight into LDS
-    __device__ __forceinline__ void stage_direct(char *lds, int src, int st, int wave) const {
+    // What the requests of one stage share.  Rows past the matrix lie past its end and arrive as zeros; k past the sum does, too, where k runs over rows, and is
+    // put there where it runs along them
+    static constexpr int BUFFERS = GATED_B && WAVES == 4 ? 2 : 1;  // eight waves: a wave's rows are all of gate or all of up
+    static_assert(!GATED_B || WAVES == 4 || WAVES == 8, "");
+    struct Request {
+        i32x4 buffer[BUFFERS];
+        unsigned off[PERIOD];
+    };
+    // stage st (src: which source of a two-part sum)
+    __device__ __forceinline__ Request request(int src, int st, bool any, int wave, int lane) const {
         const long long adv = KC ? (long long)st * 128 : (long long)st * KSTAGE * ld;
-        i32x4 rs[GATED_B ? 2 : 1];
+        long long left = end - adv;
+        left = left < 0 || !any ? 0 : left > 0x7fffffffLL ? 0x7fffffffLL : left;
+        Request r;
 #pragma unroll
-        for (int g = 0; g < (GATED_B ? 2 : 1); ++g) {
-            const int s = GATED_B ? g : src;
-            long long left = end[s] - adv;
-            left = left < 0 ? 0 : left > 0x7fffffffLL ? 0x7fffffffLL : left;
-            rs[g] = buffer_of(base[s] + adv, (int)left);
-        }
+        for (int g = 0; g < BUFFERS; ++g) r.buffer[g] = buffer_of(base[!GATED_B ? src : BUFFERS == 2 ? g : wave >> 2] + adv, (int)left);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            unsigned off;
-            bool in;
-            if constexpr (KC) {
-                off = (unsigned)row_in_source(row[i]) * (unsigned)ld + piece[i] * 16;
-                in = st * KSTAGE + piece[i] * V < k_len;
-            } else {
-                off = (unsigned)row[i] * (unsigned)ld + piece[i] * 16;
-                in = st * KSTAGE + row[i] < k_len;
-            }
-            off = in ? off : OUT_OF_RANGE;
-            const int g = GATED_B ? source_of((i * WAVES + wave) * 64 / CPR) : 0;
-            load_to_lds(rs[g], off, lds + (i * WAVES + wave) * 1024);
+        for (int t = 0; t < PERIOD; ++t) {
+            r.off[t] = (unsigned)(lane / CPR) * (unsigned)ld + piece_of(t, wave, lane) * 16;
+            if (KC && st * KSTAGE + piece_of(t, wave, lane) * V >= k_len) r.off[t] = OUT_OF_RANGE;
         }
+        return r;
+    }
+    // its i-th piece straight into LDS
+    __device__ __forceinline__ void issue(const Request &r, int i, char *lds, int wave) const {
+        const int row = (i * WAVES + wave) * RPI;
+        load_to_lds(r.buffer[BUFFERS == 2 ? i & 1 : 0], r.off[i % PERIOD] + (unsigned)row_in_source(row) * (unsigned)ld, lds + (i * WAVES + wave) * 1024);
     }
     // ... through registers, for rows that are not whole aligned pieces
-    __device__ __forceinline__ void load_regs(i32x4 *r, int src, int st) const {
+    __device__ __forceinline__ void load_regs(i32x4 *r, int src, int st, int wave, int lane) const {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int k0 = st * KSTAGE + (KC ? piece[i] * V : row[i]);
-            const int s = GATED_B ? source_of(row[i]) : src;
-            const int rr = KC ? row_in_source(row[i]) : piece[i] * V;  // first row / column
+            const int row = row_of(i, wave, lane), piece = piece_of(i, wave, lane);
+            const int k0 = st * KSTAGE + (KC ? piece * V : row);
+            const int s = GATED_B ? source_of(row) : src;
+            const int rr = KC ? row_in_source(row) : piece * V;  // first row / column
             const char *p = KC ? base[s] + (long long)rr * ld + (long long)k0 * ES : base[s] + (long long)k0 * ld + (long long)rr * ES;
             const bool line = KC ? rr < rows_left : k0 < k_len;
             const int left = line ? (KC ? k_len - k0 : rows_left - rr) : 0;
@@ -256,16 +259,17 @@ struct Operand {
         for (int i = 0; i < PIECES; ++i) *reinterpret_cast<i32x4 *>(lds + ((i * WAVES + wave) * 64 + lane) * 16) = r[i];
     }
 
-    // fragment: rows r0 + lane % 16, k of the stage's step `sub`
+    // fragment: rows r0 + lane % 32, k of the stage's step `sub`
     __device__ static __forceinline__ i32x4 fragment(const char *lds, int r0, int sub, int lane) {
-        const int i = lane & 15, g = lane >> 4;
+        const int i = lane & 31, g = lane >> 5;
         if constexpr (KC) {
             const int r = r0 + i;
-            return *reinterpret_cast<const i32x4 *>(lds + r * 128 + (((sub * 4 + g) ^ kc_swizzle(r)) << 4));
+            return *reinterpret_cast<const i32x4 *>(lds + r * 128 + (((sub * 2 + g) ^ kc_swizzle(r)) << 4));
         } else if constexpr (ES == 2) {
+            // groups of 16 lanes: lane 4 a + b points at k = a, columns 4 b .. + 3, and receives column 4 a + b, k = 0 .. 3
             typedef __attribute__((address_space(3))) i16x4 *lds_ptr;
-            const int k = sub * 32 + g * 8 + (i >> 2);
-            const char *p = lds + k * (R * 2) + (((r0 / 8 + ((i & 3) >> 1)) ^ swizzle(k)) << 4) + (i & 1) * 8;
+            const int k = sub * 16 + g * 8 + ((i & 15) >> 2), c = r0 + (i & 16) + (i & 3) * 4;
+            const char *p = lds + k * (R * 2) + (((c >> 3) ^ swizzle(k)) << 4) + (c & 4) * 2;
             const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
             const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * R * 2));
             return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -273,7 +277,7 @@ struct Operand {
             f32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int k = sub * 16 + g * 4 + j, c = r0 + i;
+                const int k = (sub * 2 + g) * 4 + j, c = r0 + i;
                 v[j] = *reinterpret_cast<const float *>(lds + k * (R * 4) + (((c >> 2) ^ swizzle(k)) << 4) + (c & 3) * 4);
             }
             return __builtin_bit_cast(i32x4, v);
@@ -294,13 +298,87 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// workgroup -> (problem, tile, split): workgroups go round-robin over the 8 XCDs, each with an L2 of its own; consecutive tiles of one XCD share
-// operand rows, eight m tiles to a group
+// 32 rows of accumulators from LDS through the epilogue.  Inside the matrix with whole quads (all of a large one) the loop is stripped of bounds, of 64-bit
+// address arithmetic and of the choice of activation: with those, instructions bound it (13 us of a tile's 43 at 16384 x 1024 x 4096).
+template <typename T, int EPI, int ACT>
+__device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mine, int m, int n, int lane) {
+    constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
+    constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR, ITER = 32 / RPI;
+    typedef typename quad<T>::type Q;
+    const int row = lane / LPR, piece = lane % LPR;
+    const long long first = (long long)m * q.N + n;
+    const unsigned at = (unsigned)row * (unsigned)q.N + piece * 4, next = (unsigned)q.N * RPI;  // elements; 32 rows < 2^31 bytes (the launcher's rule)
+    T *o0 = static_cast<T *>(q.out[0]) + first;
+    T *o1 = BWD ? static_cast<T *>(q.out[1]) + first : nullptr;
+    float *g0 = GATED && q.out[1] ? static_cast<float *>(q.out[1]) + first : nullptr, *u0 = g0 ? static_cast<float *>(q.out[2]) + first : nullptr;
+    const float *gi = BWD ? static_cast<const float *>(q.in[0]) + first : nullptr, *ui = BWD ? static_cast<const float *>(q.in[1]) + first : nullptr;
+    f32x4 g[ITER], u[ITER];
+    if constexpr (BWD) {
+#pragma unroll
+        for (int k = 0; k < ITER; ++k) {
+            g[k] = *reinterpret_cast<const f32x4 *>(gi + at + k * next);
+            u[k] = *reinterpret_cast<const f32x4 *>(ui + at + k * next);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+        const int r = k * RPI + row;
+        const unsigned o = at + k * next;
+        const f32x4 c0 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + ((piece ^ (r & 15)) << 4));
+        if constexpr (EPI == EPI_STORE) *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(c0, Q);
+        else if constexpr (GATED) {
+            const f32x4 c1 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + (((piece + 8) ^ (r & 15)) << 4));
+            f32x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = act_value<ACT>(c0[e]) * c1[e];
+            *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(h, Q);
+            if (g0) {
+                *reinterpret_cast<f32x4 *>(g0 + o) = c0;
+                *reinterpret_cast<f32x4 *>(u0 + o) = c1;
+            }
+        } else {
+            f32x4 dg, du;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float a, da;
+                act_grad<ACT>(g[k][e], a, da);
+                dg[e] = c0[e] * u[k][e] * da;
+                du[e] = c0[e] * a;
+            }
+            *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(dg, Q);
+            *reinterpret_cast<Q *>(o1 + o) = __builtin_convertvector(du, Q);
+        }
+    }
+}
+
+template <typename T, int EPI>
+__device__ __forceinline__ void rows_out(const GemmProblem &q, int act, const char *mine, int m, int n, int lane) {
+    constexpr bool GATED = EPI == EPI_GATED;
+    constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR;
+    if (q.quads && m + 32 <= q.M && n + LPR * 4 <= q.N) {
+        if (EPI == EPI_STORE || act == GD_ACT_SILU) rows_inside<T, EPI, GD_ACT_SILU>(q, mine, m, n, lane);
+        else if (act == GD_ACT_GELU) rows_inside<T, EPI, GD_ACT_GELU>(q, mine, m, n, lane);
+        else rows_inside<T, EPI, GD_ACT_GELU_TANH>(q, mine, m, n, lane);
+        return;
+    }
+    const int piece = lane % LPR;
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPI) {
+        f32x4 g = {0.f, 0.f, 0.f, 0.f}, u = g, c1 = g;
+        const f32x4 c0 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + ((piece ^ (r & 15)) << 4));
+        if constexpr (GATED) c1 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + (((piece + 8) ^ (r & 15)) << 4));
+        if constexpr (EPI == EPI_GATED_BWD) load_kept(q, m + r, n + piece * 4, g, u);
+        epilogue<T, EPI>(q, act, m + r, n + piece * 4, c0, c1, g, u);
+    }
+}
+
+// piece of work -> (problem, tile, split): workgroups go round-robin over the 8 XCDs, each with an L2 of its own (and take every gridDim-th piece, a
+// multiple of 8 further); consecutive pieces of one XCD share operand rows, eight m tiles to a group
 struct Place {
     int problem, mt, nt, split;
 };
-__device__ __forceinline__ Place place(const GemmLaunch &p) {
-    const int total = gridDim.x, id = blockIdx.x;
+__device__ __forceinline__ Place place(const GemmLaunch &p, int id) {
+    const int total = p.blocks;
     const int q = total >> 3, r = total & 7, xcd = id & 7;
     int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
     Place w;
@@ -318,198 +396,200 @@ __device__ __forceinline__ Place place(const GemmLaunch &p) {
     return w;
 }
 
+// One workgroup per CU (256 x 256 tiles) or two walk the pieces of work.  The stages of a workgroup's pieces run through the ring as one stream: behind the
+// last stage of a piece the first ones of the next are on their way, and the epilogue uses only the places of stages that have been multiplied, so neither
+// the start of a workgroup nor the way of its first stage nor the stores of the last tile are waited for.
 template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool DIRECT>
-__global__ __launch_bounds__(WM *WN * 64, 1) void gemm_kernel(const GemmLaunch p) {
+__global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p) {
     constexpr int THREADS = WM * WN * 64;
     constexpr bool GATED = EPI == EPI_GATED;
-    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-    static_assert(TN == 64 && TM % 64 == 0, "a wave's 64 columns (32 of gate and 32 of up) and groups of 64 rows go through 16 KB of LDS");
-    constexpr int STEPS = AKC || BKC || !DIRECT ? 2 : 1, RING = 4 / STEPS;
-    typedef Operand<T, BM, AKC, STEPS, THREADS, false> OpA;
-    typedef Operand<T, BN, BKC, STEPS, THREADS, GATED> OpB;
-    constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES;
-    static_assert(WM * WN * 16384 <= RING * STAGE, "");
-    constexpr int KSTAGE = OpA::KSTAGE;
-    __shared__ __attribute__((aligned(16))) char lds[RING * STAGE];
+    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    static_assert(TN == 64 && TM % 32 == 0, "a wave's 64 columns (32 of gate and 32 of up) and groups of 32 rows go through 8 KB of LDS");
+        typedef Operand<T, BM, AKC, THREADS, false> OpA;
+    typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
+    constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES, KSTAGE = OpA::KSTAGE;
+    static_assert(WM * WN * 8192 == STAGE, "the epilogue takes one place, the next piece's first stage the other");
+    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const Place w = place(p);
-    const GemmProblem &q = p.q[w.problem];
-    const int m0 = w.mt * BM, n0 = w.nt * (GATED ? BN / 2 : BN);
 
     OpA a;
     OpB b;
-    a.init(wave, lane);
-    b.init(wave, lane);
-    a.ld = q.lda; b.ld = q.ldb;
-    a.k_len = b.k_len = q.K;
-    a.rows_left = q.M - m0; b.rows_left = q.N - n0;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
+
+    // the piece whose stages are being requested
+    Place w;
+    int per_part = 0, st0 = 0, stages = 0;
+    auto open = [&](int id) __attribute__((always_inline)) {
+        w = place(p, id);
+        const GemmProblem &q = p.q[w.problem];
+        const int m0 = w.mt * BM, n0 = w.nt * (GATED ? BN / 2 : BN);
+        a.ld = q.lda; b.ld = q.ldb;
+        a.k_len = b.k_len = q.K;
+        a.rows_left = q.M - m0; b.rows_left = q.N - n0;
         const long long oa = AKC ? (long long)m0 * q.lda : (long long)m0 * sizeof(T);
         const long long ob = BKC ? (long long)n0 * q.ldb : (long long)n0 * sizeof(T);
-        a.base[s] = static_cast<const char *>(q.a[s]) + oa;
-        b.base[s] = static_cast<const char *>(q.b[s]) + ob;
-        a.end[s] = q.a_bytes - oa;
-        b.end[s] = q.b_bytes - ob;
-    }
-    const int per_part = (q.K + KSTAGE - 1) / KSTAGE;  // stages of one part of the sum
-    const int st0 = w.split * q.stages_per_split;
-    const int st1 = min(st0 + q.stages_per_split, per_part * q.parts);
-
-    f32x4 acc[FN][FM];
+        a.end = q.a_bytes - oa;
+        b.end = q.b_bytes - ob;
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < 2; ++s) {
+            a.base[s] = static_cast<const char *>(q.a[s]) + oa;
+            b.base[s] = static_cast<const char *>(q.b[s]) + ob;
+        }
+        per_part = max(1, (q.K + KSTAGE - 1) / KSTAGE);  // stages of one part of the sum (an empty sum: one stage of zeros)
+        st0 = w.split * q.stages_per_split;
+        stages = min(q.stages_per_split, per_part * q.parts - st0);
+    };
 
+    int at = 0;  // place of the current piece's stage 0
+    auto place_of = [&](int st) __attribute__((always_inline)) { return lds + ((at + st) & 1) * STAGE; };
     i32x4 ra[DIRECT ? 1 : OpA::PIECES], rb[DIRECT ? 1 : OpB::PIECES];
-    auto place_of = [&](int st) __attribute__((always_inline)) { return lds + ((st - st0) & (RING - 1)) * STAGE; };
-    auto fetch = [&](int st) __attribute__((always_inline)) {
-        const int src = st >= per_part, k = src ? st - per_part : st;
+    // stage st of the open piece: what its requests share, then its LOADS requests one by one (or, through registers, all of it)
+    typename OpA::Request qa;
+    typename OpB::Request qb;
+    auto request = [&](int st, bool any) __attribute__((always_inline)) {
+        const int src = st0 + st >= per_part, k = src ? st0 + st - per_part : st0 + st;
         if constexpr (DIRECT) {
-            a.stage_direct(place_of(st), src, k, wave);
-            b.stage_direct(place_of(st) + OpA::BYTES, src, k, wave);
+            qa = a.request(src, k, any, wave, lane);
+            qb = b.request(src, k, any, wave, lane);
         } else {
-            a.load_regs(ra, src, k);
-            b.load_regs(rb, src, k);
+            a.load_regs(ra, src, k, wave, lane);
+            b.load_regs(rb, src, k, wave, lane);
         }
     };
-    auto commit = [&](int st) __attribute__((always_inline)) {
-        a.store_regs(place_of(st), ra, wave, lane);
-        b.store_regs(place_of(st) + OpA::BYTES, rb, wave, lane);
+    auto issue = [&](int i, char *to) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+            if (i < OpA::PIECES) a.issue(qa, i, to, wave);
+            else b.issue(qb, i - OpA::PIECES, to + OpA::BYTES, wave);
+        }
     };
+    auto fetch = [&](int st, char *to) __attribute__((always_inline)) {
+        request(st, true);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) issue(i, to);
+    };
+    auto commit = [&](char *to) __attribute__((always_inline)) {
+        a.store_regs(to, ra, wave, lane);
+        b.store_regs(to + OpA::BYTES, rb, wave, lane);
+    };
+    f32x16 acc[FN][FM];
     i32x4 fa[2][FM], fb[2][FN];
     auto read = [&](int st, int sub, int set) __attribute__((always_inline)) {
-        const char *at = place_of(st);
 #pragma unroll
-        for (int i = 0; i < FN; ++i) fb[set][i] = OpB::fragment(at + OpA::BYTES, wn * TN + i * 16, sub, lane);
+        for (int i = 0; i < FN; ++i) fb[set][i] = OpB::fragment(place_of(st) + OpA::BYTES, wn * TN + i * 32, sub, lane);
 #pragma unroll
-        for (int j = 0; j < FM; ++j) fa[set][j] = OpA::fragment(at, wm * TM + j * 16, sub, lane);
+        for (int j = 0; j < FM; ++j) fa[set][j] = OpA::fragment(place_of(st), wm * TM + j * 32, sub, lane);
     };
     auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int i = 0; i < FN; ++i) acc[i][j] = mma<T>(fb[set][i], fa[set][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);  // the order stays: products cover the way of the reads before them
+    };
+
+    int id = blockIdx.x, n = 0, ahead = 0;  // n: stages of the current piece; ahead: stages of the next one that have been requested
+
+    if (id >= p.blocks) return;
+    open(id);
+    for (;;) {
+        // the current piece is open, `ahead` of its stages have been requested and have arrived
+        n = stages;
+        const GemmProblem &q = p.q[w.problem];
+        const int mw = w.mt * BM + wm * TM, nw = w.nt * (GATED ? BN / 2 : BN) + wn * (GATED ? TN / 2 : TN), split = w.split;
+#pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
-            for (int j = 0; j < FM; ++j) acc[i][j] = mma<T>(fb[set][i], fa[set][j], acc[i][j]);
-    };
-    // step `sub` of stage st, its fragments in (or on their way to) set.  At the stage's last step all its fragments have been read: behind the barrier its place
-    // is free and the next stage complete.  full: stages up to st + RING exist (no conditions in the long part of the loop)
-    auto step = [&](int st, int sub, int set, bool full) __attribute__((always_inline)) {
-        if (sub + 1 < STEPS) read(st, sub + 1, set ^ 1);
-        else if (full || st + 1 < st1) {
-            if constexpr (DIRECT) {
-                if (full || st + RING - 1 < st1) wait_loads<(RING - 2) * LOADS>();  // stages up to st + RING - 1 have been requested
-                else wait_loads<0>();
-            } else commit(st + 1);
-            lds_barrier();
-            if constexpr (DIRECT) {
-                if (full || st + RING < st1) fetch(st + RING);
-            } else {
-                if (full || st + 2 < st1) fetch(st + 2);
-            }
-            read(st + 1, 0, set ^ 1);
-        }
-        multiply(set);
-        __builtin_amdgcn_sched_barrier(0);  // the products stay between the reads and the next barrier: they cover the reads' way
-    };
-
-    if (st0 < st1) {
+            for (int j = 0; j < FM; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
         if constexpr (DIRECT) {
+            if (ahead == 0) fetch(0, place_of(0));
+            if (1 < n) fetch(1, place_of(1));
+            if (ahead == 0) {
+                if (1 < n) wait_loads<LOADS>();
+                else wait_loads<0>();
+                lds_barrier();
+            }
+        } else {
+            fetch(0, nullptr);
+            commit(place_of(0));
+            if (1 < n) fetch(1, nullptr);
+            lds_barrier();
+        }
+        ahead = 0;
+        read(0, 0, 0);
+        auto three = [&](int st) __attribute__((always_inline)) {  // a stage's first three steps
 #pragma unroll
-            for (int k = 0; k < RING; ++k)
-                if (st0 + k < st1) fetch(st0 + k);
-            if (st0 + RING <= st1) wait_loads<(RING - 1) * LOADS>();
-            else wait_loads<0>();
-        } else {
-            fetch(st0);
-            commit(st0);
-            if (st0 + 1 < st1) fetch(st0 + 1);
+            for (int sub = 0; sub < 3; ++sub) {
+                read(st, sub + 1, (sub + 1) & 1);
+                multiply(sub & 1);
+            }
+        };
+        three(0);
+        for (int st = 0; st + 1 < n; ++st) {
+            // stage st's last step, its fragments in (or on their way to) set 1: behind the barrier its place is free and the next stage complete
+            if constexpr (DIRECT) wait_loads<0>();
+            else commit(place_of(st + 1));
+            lds_barrier();
+            char *to = place_of(st);
+            if (st + 2 >= n && id + (int)gridDim.x < p.blocks && DIRECT) {
+                open(id + gridDim.x);
+                ahead = 1;
+            }
+            if (DIRECT || st + 2 < n) request(st + 2 < n ? st + 2 : 0, st + 2 < n || ahead);  // (nothing left to request: zeros into a place that nobody reads)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) issue(i, to);
+            read(st + 1, 0, 0);
+            multiply(1);
+            three(st + 1);
         }
-        lds_barrier();
-        read(st0, 0, 0);
-        int st = st0;
-        if constexpr (STEPS == 2) {
-            for (; st + RING < st1; ++st) {
-                step(st, 0, 0, true);
-                step(st, 1, 1, true);
-            }
-            for (; st < st1; ++st) {
-                step(st, 0, 0, false);
-                step(st, 1, 1, false);
-            }
-        } else {
-            for (; st + 1 + RING < st1; st += 2) {
-                step(st, 0, 0, true);
-                step(st + 1, 0, 1, true);
-            }
-            for (; st < st1; st += 2) {
-                step(st, 0, 0, false);
-                if (st + 1 < st1) step(st + 1, 0, 1, false);
-            }
-        }
-    }
+        multiply(1);
+        wait_loads<0>();
+        lds_barrier();  // every wave has read the last stage; the next piece's first ones are complete
 
-    constexpr int NI = GATED ? FN / 2 : FN;
-    const int mw = m0 + wm * TM, nw = n0 + wn * (GATED ? TN / 2 : TN);  // the wave's first row and column
-    if (q.splits == 1) {
-        // The accumulators go through LDS, 64 rows of the wave at a time (16 KB a wave, 16-byte pieces of row r at piece ^ r), and come back row by row:
-        // global memory is read and written in whole lines, and the loop over them stays a loop (unrolled over the accumulators, three activations
-        // kept the accumulators in scratch memory: dh of 16384 x 4096 x 1024 with its epilogue took 977 us, now 329).
-        constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR, ITER = 64 / RPI, BATCH = 4;
-        char *mine = lds + wave * 16384;
-        __syncthreads();  // every wave has read the last stage
+        if (q.splits == 1) {
+            // The accumulators go through LDS, 32 rows of the wave at a time (8 KB a wave, 16-byte pieces of row r at piece ^ r), and come back row by row:
+            // global memory is read and written in whole lines
+            char *mine = place_of(n - 1) + wave * 8192;
 #pragma unroll
-        for (int jc = 0; jc < FM; jc += 4) {
+            for (int j = 0; j < FM; ++j) {
+                const int r = lane & 31;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    const int r = j * 16 + (lane & 15);
-                    *reinterpret_cast<f32x4 *>(mine + r * 256 + (((i * 4 + (lane >> 4)) ^ (r & 15)) << 4)) = acc[i][jc + j];
-                }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const int piece = lane & (LPR - 1), n = nw + piece * 4;
-#pragma unroll 1
-            for (int it = 0; it < ITER; it += BATCH) {
-                f32x4 g[BATCH], u[BATCH];
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    g[k] = u[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if constexpr (EPI == EPI_GATED_BWD) load_kept(q, mw + jc * 16 + (it + k) * RPI + lane / LPR, n, g[k], u[k]);
-                }
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    const int r = (it + k) * RPI + lane / LPR;
-                    const f32x4 c0 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + ((piece ^ (r & 15)) << 4));
-                    f32x4 c1 = {0.f, 0.f, 0.f, 0.f};
-                    if constexpr (GATED) c1 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + (((piece + 8) ^ (r & 15)) << 4));
-                    epilogue<T, EPI>(q, p.act, mw + jc * 16 + r, n, c0, c1, g[k], u[k]);
-                }
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<f32x4 *>(mine + r * 256 + (((i * 8 + e * 2 + (lane >> 5)) ^ (r & 15)) << 4)) = quad_of(acc[i][j], e);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                rows_out<T, EPI>(q, p.act, mine, mw + j * 32, nw, lane);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-    } else {
-        // partial sums, rows padded to whole quads: [split][plane][M][N4]
-        const long long n4 = (q.N + 3) & ~3, plane = (long long)q.M * n4;
-        float *part = q.partial + (long long)w.split * (GATED ? 2 : 1) * plane;
-        const int nr = nw + (lane >> 4) * 4;
+        } else {
+            // partial sums, rows padded to whole quads: [split][plane][M][N4]
+            const long long n4 = (q.N + 3) & ~3, plane = (long long)q.M * n4;
+            float *part = q.partial + (long long)split * (GATED ? 2 : 1) * plane;
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int m = mw + (lane & 15) + j * 16;
-            if (m >= q.M) continue;
+            for (int j = 0; j < FM; ++j) {
+                const int m = mw + j * 32 + (lane & 31);
+                if (m >= q.M) continue;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                if (nr + i * 16 >= q.N) continue;
-                float *d = part + (long long)m * n4 + nr + i * 16;
-                *reinterpret_cast<f32x4 *>(d) = acc[i][j];
-                if constexpr (GATED) *reinterpret_cast<f32x4 *>(d + plane) = acc[(i + NI) % FN][j];
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = nw + (GATED ? 0 : i * 32) + e * 8 + (lane >> 5) * 4;
+                        if (c < q.N) *reinterpret_cast<f32x4 *>(part + (GATED ? i * plane : 0) + (long long)m * n4 + c) = quad_of(acc[i][j], e);
+                    }
             }
         }
+
+        id += gridDim.x;
+        if (id >= p.blocks) return;
+        lds_barrier();  // the epilogue's places are free
+        at = (at + n) & 1;
+        if (ahead == 0) open(id);
     }
 }
 
@@ -538,12 +618,12 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmLaunch p) {
 }
 
 template <typename T, bool AKC, bool BKC, int EPI>
-int launch_gemm(const GemmLaunch &p, int blocks, hipStream_t s) {
-    if (blocks > 0) {
+int launch_gemm(const GemmLaunch &p, hipStream_t s) {
+    if (p.blocks > 0) {
         if (p.tile == TILE_256) {
-            if constexpr (sizeof(T) == 2) gemm_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, true><<<blocks, 512, 0, s>>>(p);
-        } else if (p.direct) gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, true><<<blocks, 256, 0, s>>>(p);
-        else gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, false><<<blocks, 256, 0, s>>>(p);
+            if constexpr (sizeof(T) == 2) gemm_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, true><<<p.grid, 512, 0, s>>>(p);
+        } else if (p.direct) gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
+        else gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
         GD_HIP(hipGetLastError());
     }
     if (p.join_blocks > 0) {
@@ -554,13 +634,13 @@ int launch_gemm(const GemmLaunch &p, int blocks, hipStream_t s) {
 }
 
 template <typename T>
-int launch_type(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s) {
+int launch_type(const GemmLaunch &p, GemmKind kind, hipStream_t s) {
     switch (kind) {
-        case GEMM_GATE_UP: return launch_gemm<T, true, true, EPI_GATED>(p, blocks, s);
-        case GEMM_DOWN: return launch_gemm<T, true, true, EPI_STORE>(p, blocks, s);
-        case GEMM_DHIDDEN: return launch_gemm<T, true, false, EPI_GATED_BWD>(p, blocks, s);
-        case GEMM_DX: return launch_gemm<T, true, false, EPI_STORE>(p, blocks, s);
-        case GEMM_DW: return launch_gemm<T, false, false, EPI_STORE>(p, blocks, s);
+        case GEMM_GATE_UP: return launch_gemm<T, true, true, EPI_GATED>(p, s);
+        case GEMM_DOWN: return launch_gemm<T, true, true, EPI_STORE>(p, s);
+        case GEMM_DHIDDEN: return launch_gemm<T, true, false, EPI_GATED_BWD>(p, s);
+        case GEMM_DX: return launch_gemm<T, true, false, EPI_STORE>(p, s);
+        case GEMM_DW: return launch_gemm<T, false, false, EPI_STORE>(p, s);
     }
     return 1;
 }

@@ -84,7 +84,7 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
 long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
-    const int kstage = (kind == GEMM_DW && l.direct ? 64 : 128) / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
+    const int kstage = 128 / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
     auto tiles = [&](int t) {
         long long n = 0;
         for (int i = 0; i < l.problems; ++i) n += ((l.q[i].M + t - 1LL) / t) * ((l.q[i].N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
@@ -100,14 +100,14 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
         GemmProblem &q = l.q[i];
         q.tiles_m = (int)((q.M + t - 1LL) / t);
         q.tiles_n = (int)((q.N + (gated ? t / 2 : t) - 1LL) / (gated ? t / 2 : t));
-        const long long stages = (long long)q.parts * ((q.K + kstage - 1) / kstage);
+        const long long stages = q.K ? (long long)q.parts * ((q.K + kstage - 1) / kstage) : 1;
         // few tiles and a long sum: split it over workgroups, at least 4 stages each
         long long splits = all > 0 ? room / all : 1;
         if (splits > stages / 4) splits = stages / 4;
         if (splits > 16) splits = 16;
         if (splits < 1) splits = 1;
         q.stages_per_split = (int)((stages + splits - 1) / splits);
-        q.splits = q.stages_per_split ? (int)((stages + q.stages_per_split - 1) / q.stages_per_split) : 1;
+        q.splits = (int)((stages + q.stages_per_split - 1) / q.stages_per_split);
         q.blocks = q.tiles_m * q.tiles_n * q.splits;
         blocks += q.blocks;
         q.join_threads = 0;
@@ -120,26 +120,26 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     }
     if (blocks > (1LL << 30) || join / 256 > (1LL << 30)) return -1;
     l.join_blocks = (int)(join / 256);
+    l.blocks = (int)blocks;
+    l.grid = (int)(blocks < room ? blocks : room / 8 * 8);  // a workgroup's pieces stay on its XCD
     return floats;
 }
 
 int run_gemm(GemmLaunch &l, int dtype, GemmKind kind, float *partial, hipStream_t s, const char *who) {
     const bool gated = kind == GEMM_GATE_UP;
     GD_CHECK(plan_gemm(l, dtype, kind) >= 0, "%s: too many tiles for one launch", who);
-    int blocks = 0;
     for (int i = 0; i < l.problems; ++i) {
         GemmProblem &q = l.q[i];
-        q.quads = q.N % 4 == 0;
+        q.quads = q.N % 4 == 0 && q.N < (1 << 23);  // 32 rows of 4-byte elements stay under 2^31 bytes
         for (const void *o : {(const void *)q.out[0], (const void *)q.out[1], (const void *)q.out[2], q.in[0], q.in[1]})
             if ((uintptr_t)o % 16) q.quads = 0;
         q.partial = partial;
         if (q.splits > 1) partial += (long long)q.splits * (gated ? 2 : 1) * q.M * ((q.N + 3LL) / 4 * 4);
-        blocks += q.blocks;
     }
     switch (dtype) {
-        case GD_BF16: return launch_ffn_gemm_bf16(l, kind, blocks, s);
-        case GD_F16: return launch_ffn_gemm_f16(l, kind, blocks, s);
-        default: return launch_ffn_gemm_f32(l, kind, blocks, s);
+        case GD_BF16: return launch_ffn_gemm_bf16(l, kind, s);
+        case GD_F16: return launch_ffn_gemm_f16(l, kind, s);
+        default: return launch_ffn_gemm_f32(l, kind, s);
     }
 }
 

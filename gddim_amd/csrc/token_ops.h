@@ -67,11 +67,12 @@ struct GemmProblem {
 struct GemmLaunch {
     GemmProblem q[3];
     int problems, act, direct, join_blocks;
+    int blocks, grid;            // pieces of work; workgroups
     GemmTile tile;
 };
 
-int launch_ffn_gemm_bf16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
-int launch_ffn_gemm_f16(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
-int launch_ffn_gemm_f32(const GemmLaunch &p, GemmKind kind, int blocks, hipStream_t s);
+int launch_ffn_gemm_bf16(const GemmLaunch &p, GemmKind kind, hipStream_t s);
+int launch_ffn_gemm_f16(const GemmLaunch &p, GemmKind kind, hipStream_t s);
+int launch_ffn_gemm_f32(const GemmLaunch &p, GemmKind kind, hipStream_t s);
 
 }  // namespace gd
