@@ -84,6 +84,24 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
 long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
+    // Few rows: the weight-streaming kernel, up to 64, and further while 16 rows of x at a time do not read more of the weights than a launch costs
+    // (skinny_kernel has the figures; 96 x 1024 x 4096 would take 41 us instead of 33, 128 x 256 x 688 takes 8.2 instead of 19.6)
+    if ((kind == GEMM_GATE_UP || kind == GEMM_DOWN) && l.direct && l.q[0].M <= 256) {
+        GemmProblem &q = l.q[0];
+        const int m_tiles = (q.M + 15) / 16;
+        if (q.M <= 64 || (long long)m_tiles * (gated ? 2 : 1) * q.N * q.K * (long long)elem_size(dtype) <= (12LL << 20)) {
+            l.tile = TILE_SKINNY;
+            q.splits = 1;
+            q.tiles_m = m_tiles;
+            l.skinny_rows = 16;
+            while (l.skinny_rows > 4 && 2LL * m_tiles * ((q.N + l.skinny_rows - 1) / l.skinny_rows) <= cus) l.skinny_rows /= 2;
+            const long long grid = (q.N + 8LL * l.skinny_rows - 1) / (8LL * l.skinny_rows) * 8 * m_tiles;
+            if (grid > (1LL << 30)) return -1;
+            l.grid = l.blocks = (int)grid;
+            l.join_blocks = 0;
+            return 0;
+        }
+    }
     const int kstage = 128 / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
     auto tiles = [&](int t) {
         long long n = 0;

@@ -46,7 +46,7 @@ int launch_rotary(RotaryParams p, int dtype, RotaryMode mode, void *dw0, void *d
 // ---- gated feed-forward block (kernels/gated_ffn_gemm.h) ----
 enum GemmKind { GEMM_GATE_UP, GEMM_DOWN, GEMM_DHIDDEN, GEMM_DX, GEMM_DW };
 enum GemmEpilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD };
-enum GemmTile { TILE_128, TILE_256 };
+enum GemmTile { TILE_128, TILE_256, TILE_SKINNY };
 
 // C[m][n] = sum over parts and k of A[m][k] B[n][k]
 struct GemmProblem {
@@ -68,6 +68,7 @@ struct GemmLaunch {
     GemmProblem q[3];
     int problems, act, direct, join_blocks;
     int blocks, grid;            // pieces of work; workgroups
+    int skinny_rows;             // TILE_SKINNY: rows of the weights a workgroup takes
     GemmTile tile;
 };
 

@@ -5,6 +5,7 @@ Tensors are float32, bfloat16 or float16 and stay in their type; work is queued 
 synchronises, and every call can be captured into a graph.  The operators record no autograd graph: gradients come from the *_backward calls, and a
 tensor that requires grad is refused while grad mode is on.  No reference counterpart."""
 import ctypes
+import functools
 import math
 
 from . import _abi
@@ -22,6 +23,26 @@ def _torch():
     return _TORCH
 
 
+def _raw_stream(index):
+    """hipStream_t of a device's current stream (torch's own short way where it has one: the public one builds two objects for a small call's 1.9 us)"""
+    torch = _torch()[0]
+    short = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return short(index) if short is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(t, fn, *args):
+    """fn(*args, stream) on t's device and its current stream, whatever device is current"""
+    torch = _torch()[0]
+    index = t.get_device()
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc)
+
+
 def _on_gpu(t, name):
     torch = _torch()[0]
     if not isinstance(t, torch.Tensor):
@@ -37,24 +58,6 @@ def _like(t, name, ref, ref_name):
     _on_gpu(t, name)
     if t.dtype != ref.dtype or t.device != ref.device:
         raise GddimError("%s is %s on %s, %s is %s on %s: types and devices must agree" % (name, t.dtype, t.device, ref_name, ref.dtype, ref.device))
-
-
-class _Device:
-    """The tensors' device made current for a native call (a no-op when it is)."""
-
-    def __init__(self, t):
-        torch = _torch()[0]
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-        self.t = t
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return ctypes.c_void_p(_torch()[0].cuda.current_stream(self.t.device).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
 
 
 class RotaryAxes:
@@ -107,10 +110,13 @@ def _check_heads(t, name, like=None, like_name=None):
 def _new(t):
     """An output like t: its order of dimensions where t is dense with adjacent channels ((B, heads, N, D) seen as (B, N, heads, D)), else contiguous."""
     torch = _torch()[0]
-    if t.is_contiguous() or 0 in t.stride() or 0 in t.shape:
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    out = torch.empty_like(t)
-    return out if out.stride(3) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    if 0 not in t.stride():
+        out = torch.empty_like(t)
+        if out.stride(3) == 1:
+            return out
+    return t.new_empty(t.shape)
 
 
 def _rotary_desc(x, pos, axes):
@@ -149,8 +155,7 @@ def rotary(x, pos, axes, inverse=False):
     out = _new(x)
     x, xv = _heads(x, "x")
     _, ov = _heads(out, "out")
-    with _Device(x) as stream:
-        check(_abi.lib().gd_rotary(desc, xv, ov, x.shape[2], int(bool(inverse)), stream))
+    _call(x, _abi.lib().gd_rotary, desc, xv, ov, x.shape[2], int(bool(inverse)))
     return out
 
 
@@ -192,10 +197,8 @@ def qk_norm_rotary(q, k, weight_q, weight_k, pos, axes, eps=1e-6):
     desc = _rotary_desc(q, pos, axes)
     qo, ko = _new(q), _new(k)
     (q, qv), (k, kv) = _heads(q, "q"), _heads(k, "k")
-    with _Device(q) as stream:
-        check(_abi.lib().gd_qk_norm_rotary(desc, qv, kv, _heads(qo, "q")[1], _heads(ko, "k")[1], q.shape[2], k.shape[2],
-                                           w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None,
-                                           _w_f32(q, w_q, w_k), float(eps), stream))
+    _call(q, _abi.lib().gd_qk_norm_rotary, desc, qv, kv, _heads(qo, "q")[1], _heads(ko, "k")[1], q.shape[2], k.shape[2],
+          w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None, _w_f32(q, w_q, w_k), float(eps))
     return qo, ko
 
 
@@ -213,12 +216,10 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes,
     dwq, dwk = (torch.empty_like(w) if w is not None else None for w in (w_q, w_k))
     (q, qv), (k, kv), (dq_out, gqv), (dk_out, gkv) = _heads(q, "q"), _heads(k, "k"), _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
     lib = _abi.lib()
-    ws = torch.empty(lib.gd_qk_norm_rotary_backward_workspace(q.shape[3]), dtype=torch.uint8, device=q.device)
-    with _Device(q) as stream:
-        check(lib.gd_qk_norm_rotary_backward(desc, gqv, gkv, qv, kv, _heads(dq, "dq")[1], _heads(dk, "dk")[1], q.shape[2], k.shape[2],
-                                             w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None,
-                                             _w_f32(q, w_q, w_k), float(eps), ws.data_ptr(),
-                                             dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None, stream))
+    ws = q.new_empty(lib.gd_qk_norm_rotary_backward_workspace(q.shape[3]), dtype=torch.uint8)
+    _call(q, lib.gd_qk_norm_rotary_backward, desc, gqv, gkv, qv, kv, _heads(dq, "dq")[1], _heads(dk, "dk")[1], q.shape[2], k.shape[2],
+          w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None, _w_f32(q, w_q, w_k), float(eps), ws.data_ptr(),
+          dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None)
     return dq, dk, dwq, dwk
 
 
@@ -228,7 +229,8 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 def _rows(t, columns):
     """t (..., columns) as a matrix with adjacent columns and rows at least a row apart: a view where there is one"""
-    t = t.reshape(-1, columns)
+    if t.dim() != 2:
+        t = t.reshape(-1, columns)
     if (columns > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < columns):
         t = t.contiguous()
     return t
@@ -258,11 +260,20 @@ def _check_ffn(x, w_gate, w_up, w_down, act):
     return x2, w_gate, w_up, w_down, desc
 
 
-def _workspace(desc, backward, device):
-    n = _abi.lib().gd_gated_ffn_workspace(desc, backward)
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(dtype, rows, in_, hidden, out, backward, device):
+    """gd_gated_ffn_workspace of these sizes on this device (its compute units count)"""
+    desc = FfnDesc(dtype, 0, rows, in_, hidden, out, in_, in_, hidden)
+    with _torch()[0].cuda.device(device):
+        n = _abi.lib().gd_gated_ffn_workspace(desc, backward)
     if n < 0:
         check(1)
-    return _torch()[0].empty(n, dtype=_torch()[0].uint8, device=device) if n else None
+    return n
+
+
+def _workspace(x, d, backward):
+    n = _workspace_bytes(d.dtype, d.rows, d.in_, d.hidden, d.out, backward, x.get_device())
+    return x.new_empty(n, dtype=_torch()[0].uint8) if n else None
 
 
 def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
@@ -273,13 +284,11 @@ def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
     shape = x.shape[:-1] if isinstance(x, torch.Tensor) else ()
     x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
     M, F = x.shape[0], w_gate.shape[0]
-    y = torch.empty((M, w_down.shape[0]), dtype=x.dtype, device=x.device)
-    hidden = torch.empty((M, F), dtype=x.dtype, device=x.device)
-    gate, up = (torch.empty((M, F), dtype=torch.float32, device=x.device) for _ in range(2)) if save else (None, None)
-    with _Device(x) as stream:
-        ws = _workspace(desc, 0, x.device)
-        check(_abi.lib().gd_gated_ffn(desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
-                                      up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws.data_ptr() if ws is not None else None, stream))
+    y, hidden = x.new_empty((M, w_down.shape[0])), x.new_empty((M, F))
+    gate, up = (x.new_empty((M, F), dtype=torch.float32) for _ in range(2)) if save else (None, None)
+    ws = _workspace(x, desc, 0)
+    _call(x, _abi.lib().gd_gated_ffn, desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
+          up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws.data_ptr() if ws is not None else None)
     y = y.view(*shape, w_down.shape[0])
     return (y, (gate, up, hidden)) if save else y
 
@@ -304,11 +313,9 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
             raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
     dy = _rows(dy, O)
     gate, up, hidden = saved
-    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)
-    dx, dwg, dwu, dwd = new(M, D), new(F, D), new(F, D), new(O, F)
-    with _Device(x) as stream:
-        ws = _workspace(desc, 1, x.device)
-        check(_abi.lib().gd_gated_ffn_backward(desc, dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                                               gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(),
-                                               dwd.data_ptr(), ws.data_ptr() if ws is not None else None, stream))
+    dx, dwg, dwu, dwd = x.new_empty((M, D)), x.new_empty((F, D)), x.new_empty((F, D)), x.new_empty((O, F))
+    ws = _workspace(x, desc, 1)
+    _call(x, _abi.lib().gd_gated_ffn_backward, desc, dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+          gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr(),
+          ws.data_ptr() if ws is not None else None)
     return dx.view(shape), dwg, dwu, dwd
