@@ -56,7 +56,7 @@ def _on_gpu(t, name):
 
 def _like(t, name, ref, ref_name):
     _on_gpu(t, name)
-    if t.dtype != ref.dtype or t.device != ref.device:
+    if t.dtype is not ref.dtype or t.get_device() != ref.get_device():
         raise GddimError("%s is %s on %s, %s is %s on %s: types and devices must agree" % (name, t.dtype, t.device, ref_name, ref.dtype, ref.device))
 
 
@@ -88,14 +88,19 @@ class RotaryAxes:
         if tuple(self.frequencies.shape) != (sum(self.sections) // 2,):
             raise GddimError("RotaryAxes: frequencies of shape %s, expected (%d,)" % (tuple(self.frequencies.shape), sum(self.sections) // 2))
         self.device = device
+        self._rotated = sum(self.sections)
+        self._index = device.index if device.type == "cuda" else -1
+        self._halves = int(paired == "halves")
+        self._table = self.frequencies.data_ptr()
         self._section = (ctypes.c_int * _abi.GD_MAX_AXES)(*self.sections)
 
 
-def _heads(t, name):
+def _heads(t):
     """(tensor, its view): channels adjacent, (B, N, heads, D)"""
-    if t.stride(3) != 1 and t.shape[3] > 1:
-        t = t.contiguous()
     s = t.stride()
+    if s[3] != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+        s = t.stride()
     return t, Heads(t.data_ptr(), s[0], s[1], s[2])
 
 
@@ -120,29 +125,32 @@ def _new(t):
 
 
 def _rotary_desc(x, pos, axes):
-    torch, types, pos_types = _torch()
+    _, types, pos_types = _torch()
     if not isinstance(axes, RotaryAxes):
         raise GddimError("axes: expected a RotaryAxes, got %s" % type(axes).__name__)
     B, N, _, D = x.shape
     _on_gpu(pos, "pos")
-    if pos.dtype not in pos_types:
+    kind = pos_types.get(pos.dtype)
+    if kind is None:
         raise GddimError("pos is %s; int32, int64 and float32 positions are supported" % pos.dtype)
-    if pos.device != x.device or axes.device != x.device:
+    index = x.get_device()
+    if pos.get_device() != index or axes._index != index:
         raise GddimError("tensors on %s, positions on %s, axes on %s: devices must agree" % (x.device, pos.device, axes.device))
     A = len(axes.sections)
     ps, st = tuple(pos.shape), pos.stride()
     if ps == (N, A):
-        st = (0,) + st
+        sb, sn, sa = 0, st[0], st[1]
+    elif ps == (B, N, A):
+        sb, sn, sa = st
     elif ps == (1, N, A):
-        st = (0,) + st[1:]
-    elif ps != (B, N, A):
+        sb, sn, sa = 0, st[1], st[2]
+    else:
         raise GddimError("pos has shape %s, expected (%d, %d) or (%d, %d, %d)" % (ps, N, A, B, N, A))
-    if sum(axes.sections) > D:
-        raise GddimError("sections %r of %d channels exceed the head's %d" % (axes.sections, sum(axes.sections), D))
+    if axes._rotated > D:
+        raise GddimError("sections %r of %d channels exceed the head's %d" % (axes.sections, axes._rotated, D))
     if B * N >= 1 << 31:
         raise GddimError("%d x %d tokens do not fit 31 bits" % (B, N))
-    return RotaryDesc(types[x.dtype], B, N, D, A, axes._section, axes.paired == "halves", pos_types[pos.dtype], pos.data_ptr(), st[0], st[1], st[2],
-                      axes.frequencies.data_ptr())
+    return RotaryDesc(types[x.dtype], B, N, D, A, axes._section, axes._halves, kind, pos.data_ptr(), sb, sn, sa, axes._table)
 
 
 def rotary(x, pos, axes, inverse=False):
@@ -153,52 +161,48 @@ def rotary(x, pos, axes, inverse=False):
     _check_heads(x, "x")
     desc = _rotary_desc(x, pos, axes)
     out = _new(x)
-    x, xv = _heads(x, "x")
-    _, ov = _heads(out, "out")
+    x, xv = _heads(x)
+    _, ov = _heads(out)
     _call(x, _abi.lib().gd_rotary, desc, xv, ov, x.shape[2], int(bool(inverse)))
     return out
 
 
 def _norm_weight(w, name, q):
-    """(pointer, is it float32 beside another type)"""
-    torch = _torch()[0]
     if w is None:
         return None
     _on_gpu(w, name)
     if tuple(w.shape) != (q.shape[3],):
         raise GddimError("%s has shape %s, expected (%d,)" % (name, tuple(w.shape), q.shape[3]))
-    if w.device != q.device or w.dtype not in (q.dtype, torch.float32):
+    if w.get_device() != q.get_device() or w.dtype is not q.dtype and w.dtype is not _torch()[0].float32:
         raise GddimError("%s is %s on %s; the tensors' type %s or float32, on %s, is supported" % (name, w.dtype, w.device, q.dtype, q.device))
     return w.contiguous()
 
 
 def _check_qk(q, k, w_q, w_k, eps):
+    """(weight_q, weight_k, their addresses, are they float32 beside another type)"""
     _check_heads(q, "q")
     _check_heads(k, "k", q, "q")
-    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise GddimError("q %s and k %s must agree in all but their heads" % (tuple(q.shape), tuple(k.shape)))
+    qs, ks = q.shape, k.shape
+    if qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
+        raise GddimError("q %s and k %s must agree in all but their heads" % (tuple(qs), tuple(ks)))
     if not (0.0 <= eps < math.inf):
         raise GddimError("eps=%r must be finite and not negative" % (eps,))
     w_q, w_k = _norm_weight(w_q, "weight_q", q), _norm_weight(w_k, "weight_k", q)
-    if w_q is not None and w_k is not None and w_q.dtype != w_k.dtype:
+    if w_q is not None and w_k is not None and w_q.dtype is not w_k.dtype:
         raise GddimError("weight_q is %s, weight_k %s: their types must agree" % (w_q.dtype, w_k.dtype))
-    return w_q, w_k
-
-
-def _w_f32(q, w_q, w_k):
     w = w_q if w_q is not None else w_k
-    return int(w is not None and w.dtype != q.dtype)
+    return (w_q, w_k, w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None,
+            int(w is not None and w.dtype is not q.dtype))
 
 
 def qk_norm_rotary(q, k, weight_q, weight_k, pos, axes, eps=1e-6):
     """RMS norms of queries and keys for each head, then the rotation, in one pass: q (B, N, heads, D) and k (B, N, key heads, D), views of a
     packed projection among them, weights (D,) of their type or float32 (None: ones).  Returns (q', k')."""
-    w_q, w_k = _check_qk(q, k, weight_q, weight_k, eps)
+    w_q, w_k, p_q, p_k, w_f32 = _check_qk(q, k, weight_q, weight_k, eps)
     desc = _rotary_desc(q, pos, axes)
     qo, ko = _new(q), _new(k)
-    (q, qv), (k, kv) = _heads(q, "q"), _heads(k, "k")
-    _call(q, _abi.lib().gd_qk_norm_rotary, desc, qv, kv, _heads(qo, "q")[1], _heads(ko, "k")[1], q.shape[2], k.shape[2],
-          w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None, _w_f32(q, w_q, w_k), float(eps))
+    (q, qv), (k, kv) = _heads(q), _heads(k)
+    _call(q, _abi.lib().gd_qk_norm_rotary, desc, qv, kv, _heads(qo)[1], _heads(ko)[1], q.shape[2], k.shape[2], p_q, p_k, w_f32, eps)
     return qo, ko
 
 
@@ -206,7 +210,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes,
     """Gradients of qk_norm_rotary: (dq, dk, dweight_q, dweight_k) from those of its outputs (None for a weight that is None).  The same bits
     every time."""
     torch = _torch()[0]
-    w_q, w_k = _check_qk(q, k, weight_q, weight_k, eps)
+    w_q, w_k, p_q, p_k, w_f32 = _check_qk(q, k, weight_q, weight_k, eps)
     for g, name, t in ((dq_out, "dq_out", q), (dk_out, "dk_out", k)):
         _check_heads(g, name, q, "q")
         if g.shape != t.shape:
@@ -214,11 +218,10 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes,
     desc = _rotary_desc(q, pos, axes)
     dq, dk = _new(q), _new(k)
     dwq, dwk = (torch.empty_like(w) if w is not None else None for w in (w_q, w_k))
-    (q, qv), (k, kv), (dq_out, gqv), (dk_out, gkv) = _heads(q, "q"), _heads(k, "k"), _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
+    (q, qv), (k, kv), (dq_out, gqv), (dk_out, gkv) = _heads(q), _heads(k), _heads(dq_out), _heads(dk_out)
     lib = _abi.lib()
     ws = q.new_empty(lib.gd_qk_norm_rotary_backward_workspace(q.shape[3]), dtype=torch.uint8)
-    _call(q, lib.gd_qk_norm_rotary_backward, desc, gqv, gkv, qv, kv, _heads(dq, "dq")[1], _heads(dk, "dk")[1], q.shape[2], k.shape[2],
-          w_q.data_ptr() if w_q is not None else None, w_k.data_ptr() if w_k is not None else None, _w_f32(q, w_q, w_k), float(eps), ws.data_ptr(),
+    _call(q, lib.gd_qk_norm_rotary_backward, desc, gqv, gkv, qv, kv, _heads(dq)[1], _heads(dk)[1], q.shape[2], k.shape[2], p_q, p_k, w_f32, eps, ws.data_ptr(),
           dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None)
     return dq, dk, dwq, dwk
 
@@ -229,6 +232,8 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 def _rows(t, columns):
     """t (..., columns) as a matrix with adjacent columns and rows at least a row apart: a view where there is one"""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.dim() != 2:
         t = t.reshape(-1, columns)
     if (columns > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < columns):
@@ -237,27 +242,27 @@ def _rows(t, columns):
 
 
 def _check_ffn(x, w_gate, w_up, w_down, act):
+    """(x as a matrix, the weights with adjacent columns, the call's description)"""
     _on_gpu(x, "x")
-    if act not in _ACTS:
+    code, kind = _torch()[1].get(x.dtype), _ACTS.get(act)
+    if kind is None:
         raise GddimError("act=%r, expected one of %s" % (act, sorted(_ACTS)))
-    if x.dtype not in _torch()[1]:
+    if code is None:
         raise GddimError("x is %s; float32, bfloat16 and float16 are supported" % x.dtype)
-    for w, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
-        _like(w, name, x, "x")
-        if w.dim() != 2:
-            raise GddimError("%s has shape %s, expected two dimensions" % (name, tuple(w.shape)))
-    if x.dim() < 1 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0] or 0 in w_gate.shape or w_down.shape[0] == 0:
-        raise GddimError("x %s, w_gate %s, w_up %s, w_down %s do not fit (..., in), (hidden, in), (hidden, in), (out, hidden)" % (
-            tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
-    w_gate, w_up, w_down = _rows(w_gate, w_gate.shape[1]), _rows(w_up, w_up.shape[1]), _rows(w_down, w_down.shape[1])
-    if w_gate.stride(0) != w_up.stride(0):
-        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
-    x2 = _rows(x, x.shape[-1])
-    if max(x2.shape[0], *w_gate.shape, w_down.shape[0]) > 1 << 30:
-        raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (x2.shape[0], x2.shape[1], w_gate.shape[0], w_down.shape[0]))
-    desc = FfnDesc(_torch()[1][x.dtype], _ACTS[act], x2.shape[0], x2.shape[1], w_gate.shape[0], w_down.shape[0], x2.stride(0), w_gate.stride(0),
-                   w_down.stride(0))
-    return x2, w_gate, w_up, w_down, desc
+    _like(w_gate, "w_gate", x, "x")
+    _like(w_up, "w_up", x, "x")
+    _like(w_down, "w_down", x, "x")
+    xs, gs, us, ds = tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)
+    if not xs or len(gs) != 2 or len(ds) != 2 or gs != us or gs[1] != xs[-1] or ds[1] != gs[0] or 0 in gs or ds[0] == 0:
+        raise GddimError("x %s, w_gate %s, w_up %s, w_down %s do not fit (..., in), (hidden, in), (hidden, in), (out, hidden)" % (xs, gs, us, ds))
+    x, w_gate, w_up, w_down = _rows(x, gs[1]), _rows(w_gate, gs[1]), _rows(w_up, gs[1]), _rows(w_down, gs[0])
+    ld = w_gate.stride(0)
+    if ld != w_up.stride(0):
+        w_gate, w_up, ld = w_gate.contiguous(), w_up.contiguous(), gs[1]
+    rows = x.shape[0]
+    if rows > 1 << 30 or gs[0] > 1 << 30 or gs[1] > 1 << 30 or ds[0] > 1 << 30:
+        raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (rows, gs[1], gs[0], ds[0]))
+    return x, w_gate, w_up, w_down, FfnDesc(code, kind, rows, gs[1], gs[0], ds[0], x.stride(0), ld, w_down.stride(0))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -280,16 +285,14 @@ def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
     """Gated feed-forward block (act(x w_gate^T) * (x w_up^T)) w_down^T: x (..., in), weights as torch.nn.Linear keeps them -- w_gate and w_up
     (hidden, in), w_down (out, hidden) -- act 'silu', 'gelu' or 'gelu_tanh'.  Returns y (..., out); with save=True (y, saved), saved for
     gated_ffn_backward (the two projections in float32 and their product).  Both projections, the activation and the product are one kernel."""
-    torch = _torch()[0]
-    shape = x.shape[:-1] if isinstance(x, torch.Tensor) else ()
+    shape = x.shape if isinstance(x, _torch()[0].Tensor) else ()
     x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
-    M, F = x.shape[0], w_gate.shape[0]
-    y, hidden = x.new_empty((M, w_down.shape[0])), x.new_empty((M, F))
-    gate, up = (x.new_empty((M, F), dtype=torch.float32) for _ in range(2)) if save else (None, None)
-    ws = _workspace(x, desc, 0)
+    y, hidden, ws = x.new_empty((desc.rows, desc.out)), x.new_empty((desc.rows, desc.hidden)), _workspace(x, desc, 0)
+    gate, up = (x.new_empty((desc.rows, desc.hidden), dtype=_torch()[0].float32) for _ in range(2)) if save else (None, None)
     _call(x, _abi.lib().gd_gated_ffn, desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
           up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws.data_ptr() if ws is not None else None)
-    y = y.view(*shape, w_down.shape[0])
+    if len(shape) != 2:
+        y = y.view(*shape[:-1], desc.out)
     return (y, (gate, up, hidden)) if save else y
 
 
