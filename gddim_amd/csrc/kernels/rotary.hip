@@ -8,14 +8,21 @@
 // All three are bound by HBM: each element is read once and written once (the gradient: two reads, one write), everything between stays in
 // registers.  What would cost more than the bytes is the angle: far positions times a frequency need 64 bits before the whole turns are
 // taken off.  One wave therefore takes a token -- or, with few tokens, a share of a token's heads -- computes the R/2 cosines and sines ONCE
-// (lane p pair p) into a table of its own in LDS, and walks the token's query and key heads with them.
+// (lane p pair p) into a table of its own in LDS, and walks the token's query and key heads with them.  A token has few heads (20 heads of 128
+// channels are three steps of a wave), so what a token begins with is read while the one before it is worked on: its positions, and behind the last heads of
+// the one its first (79 -> 45 us for the norm of 16 + 4 heads of 128 channels at 16382 tokens in bf16, with the sums below as lane permutes and one
+// hardware root a head).
 //
 // Layout: a lane holds W pairs = two vectors of W channels.  (i, i + R/2) pairs: vector 0 from the first half, vector 1 from the second;
-// (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head, so norm weights
-// and the weight-gradient sums stay in registers.  LP lanes (a power of two) hold a head: the norm's sums are log2 LP shuffles, 64 / LP heads
-// are in flight per wave.  Channels that pass through are pairs with phi = 0.
+// (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head: the weight-gradient sums stay in
+// registers (norm weights come from LDS, queries and keys apart).  LP lanes (a power of two) hold a head: the norm's sums are log2 LP permutes, 64 / LP
+// heads are in flight per wave.  Channels that pass through are pairs with phi = 0.
 //
-// W is 16 bytes of a type where pairs, strides and addresses allow it, 8 bytes else, one pair where nothing is aligned.
+// W is 16 bytes of a type where pairs, strides and addresses allow it (the gradient in 16-bit types: 8), 8 bytes else, one pair where nothing is aligned.
+//
+// Measured, against the bytes at the 5.1 TB/s of a large copy: rotation of 46800 x 16 x 128 bf16 (383 MB) 78 us, 4.9 TB/s; norm and rotation of 65536 tokens x
+// (4 + 4) x 64 float32 (268 MB) 52 us, 5.1 TB/s; of 16382 x (16 + 4) x 128 bf16 45 us, 3.7 TB/s, and its gradient (252 MB) 69 us, 3.7 TB/s, + 5 us for
+// the weights' sums.
 #include "../common.h"
 #include "../token_ops.h"
 
@@ -66,20 +73,50 @@ __device__ __forceinline__ double load_pos(const RotaryParams &p, int b, int n, 
     return (double)static_cast<const float *>(p.pos)[o];
 }
 
+// sum over the 2^lp_log2 lanes of a head: within 16 lanes by lane permutes in the adder's own operand, beyond by shuffles
+template <int CTRL> __device__ __forceinline__ float permuted(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float head_sum(float v, int lp_log2) {
+    if (lp_log2 > 0) v += permuted<0xb1>(v);   // lanes 1 0 3 2 of four
+    if (lp_log2 > 1) v += permuted<0x4e>(v);   // 2 3 0 1
+    if (lp_log2 > 2) v += permuted<0x141>(v);  // 7 .. 0 of eight: the other four
+    if (lp_log2 > 3) v += permuted<0x140>(v);  // 15 .. 0 of sixteen: the other eight
+    if (lp_log2 > 4) v += __shfl_xor(v, 16);
+    if (lp_log2 > 5) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// v^-1/2 of the hardware (one step of float32), also where v is subnormal
+__device__ __forceinline__ float inverse_root(float v) {
+    const bool tiny = v < 1e-30f;
+    return __builtin_amdgcn_rsqf(tiny ? v * 0x1p100f : v) * (tiny ? 0x1p50f : 1.f);
+}
+
 // NC: chunks of W pairs per lane (1 unless one head needs more than 64 lanes)
 template <typename T, int W, int NC, bool HALVES, int MODE>
-__global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const int lp_log2) {
+__global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void rotary_kernel(const RotaryParams p, const int lp_log2) {
     constexpr bool NORM = MODE != ROT_PLAIN, BWD = MODE == ROT_NORM_BWD;
-    extern __shared__ __attribute__((aligned(16))) float2 table_all[];
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
     const int LP = 1 << lp_log2;
     const int pairs = (p.D + 1) / 2, R2 = p.R / 2;
     const int chunks = (pairs + W - 1) / W;  // W > 1: whole (the launcher's rule)
-    float2 *table = table_all + wave * (chunks * W);
+    float2 *table = reinterpret_cast<float2 *>(smem) + wave * (chunks * W);
+    const int wpad = (p.D + 3) & ~3;
+    float *weights = reinterpret_cast<float *>(smem + (size_t)waves * chunks * W * sizeof(float2));  // [2][wpad], float32
     const int sub = lane >> lp_log2;
     const int row_step = 64 >> lp_log2;
+
+    if constexpr (NORM) {
+        for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
+            const int s = i >= p.D, e = s ? i - p.D : i;
+            weights[s * wpad + e] = !p.w[s] ? 1.f : p.w_f32 ? static_cast<const float *>(p.w[s])[e] : (float)static_cast<const T *>(p.w[s])[e];
+        }
+        __syncthreads();
+    }
 
     // this lane's channels: e0[c] .. + W - 1 and e1[c] .. + W - 1
     int e0[NC], e1[NC], ch[NC];
@@ -94,64 +131,86 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
         on0[c] = ch[c] < chunks;
         on1[c] = on0[c] && e1[c] < p.D;  // an odd head has one channel without a partner (W == 1)
     }
-    float w[2][NC][2 * W], dw[2][NC][2 * W];
-    if constexpr (NORM) {
+    float dw[2][NC][2 * W];
+    if constexpr (BWD)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 2 * W; ++i) {
-                    const int e = i < W ? e0[c] + i : e1[c] + i - W;
-                    const bool on = (i < W ? on0[c] : on1[c]) && p.heads[s];
-                    w[s][c][i] = 1.f;
-                    if (on && p.w[s]) w[s][c][i] = p.w_f32 ? static_cast<const float *>(p.w[s])[e] : (float)static_cast<const T *>(p.w[s])[e];
-                    dw[s][c][i] = 0.f;
-                }
-    }
+                for (int i = 0; i < 2 * W; ++i) dw[s][c][i] = 0.f;
     const float inv_d = 1.f / (float)p.D;
     const int rows = p.heads[0] + p.heads[1];
 
-    for (unsigned item = blockIdx.x * waves + wave; item < p.items; item += gridDim.x * waves) {
-        const int token = (int)(item / (unsigned)p.items_per_token);
-        const int share = (int)item - token * p.items_per_token;
-        const int b = token / p.tokens, n = token - b * p.tokens;
-        const int r_end = min(rows, (share + 1) * p.rows_per_item);
-
-        vec<T, W> v0[NC], v1[NC], g0[NC], g1[NC];
-        auto offset = [&](const HeadsView *hv, int r) __attribute__((always_inline)) {
-            const int seg = r >= p.heads[0];
-            const HeadsView &h = hv[seg];
-            return static_cast<T *>(h.p) + (b * h.sb + n * h.sn + (r - (seg ? p.heads[0] : 0)) * h.sh);
-        };
-        auto load = [&](int r) __attribute__((always_inline)) {
-            const T *src = offset(p.x, r);
-            const T *gsrc = BWD ? offset(p.dy, r) : nullptr;
+    // an item: a token (b, n) and the heads [r0, r_end) of it
+    struct Item {
+        int b, n, r0, r_end;
+    };
+    auto locate = [&](unsigned id) __attribute__((always_inline)) {
+        Item t;
+        const int token = (int)(id / (unsigned)p.items_per_token);
+        t.b = token / p.tokens;
+        t.n = token - t.b * p.tokens;
+        t.r0 = ((int)id - token * p.items_per_token) * p.rows_per_item;
+        t.r_end = min(rows, t.r0 + p.rows_per_item);
+        return t;
+    };
+    auto axis_of = [&](int pr) __attribute__((always_inline)) {
+        int a = 0;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                v0[c] = vec<T, W>{}; v1[c] = vec<T, W>{};
-                if (on0[c]) v0[c] = *reinterpret_cast<const vec<T, W> *>(src + e0[c]);
-                if (on1[c]) v1[c] = *reinterpret_cast<const vec<T, W> *>(src + e1[c]);
-                if constexpr (BWD) {
-                    g0[c] = vec<T, W>{}; g1[c] = vec<T, W>{};
-                    if (on0[c]) g0[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e0[c]);
-                    if (on1[c]) g1[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e1[c]);
-                }
-            }
-        };
-        int r = share * p.rows_per_item + sub;
-        if (r < r_end) load(r);  // in flight while the angles are computed
+        for (int i = 0; i < ROT_MAX_AXES - 1; ++i) a += (i + 1 < p.n_axes && pr >= p.axis_end[i]);
+        return a;
+    };
+    // the lane's first pair keeps its frequency, and its position is read an item ahead
+    const int axis0 = axis_of(lane);
+    const double freq0 = lane < R2 ? p.freq[lane] : 0.0;
+    auto pos_of = [&](const Item &t) __attribute__((always_inline)) { return lane < R2 ? load_pos(p, t.b, t.n, axis0) : 0.0; };
 
+    vec<T, W> v0[NC], v1[NC], g0[NC], g1[NC];
+    auto at = [&](const HeadsView *hv, const Item &t, int r) __attribute__((always_inline)) {
+        const int seg = r >= p.heads[0];
+        const HeadsView &h = hv[seg];
+        return static_cast<T *>(h.p) + (t.b * h.sb + t.n * h.sn + (r - (seg ? p.heads[0] : 0)) * h.sh);
+    };
+    auto load = [&](const Item &t, int r) __attribute__((always_inline)) {
+        const T *src = at(p.x, t, r);
+        const T *gsrc = BWD ? at(p.dy, t, r) : nullptr;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            v0[c] = vec<T, W>{}; v1[c] = vec<T, W>{};
+            if (on0[c]) v0[c] = *reinterpret_cast<const vec<T, W> *>(src + e0[c]);
+            if (on1[c]) v1[c] = *reinterpret_cast<const vec<T, W> *>(src + e1[c]);
+            if constexpr (BWD) {
+                g0[c] = vec<T, W>{}; g1[c] = vec<T, W>{};
+                if (on0[c]) g0[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e0[c]);
+                if (on1[c]) g1[c] = *reinterpret_cast<const vec<T, W> *>(gsrc + e1[c]);
+            }
+        }
+    };
+
+    unsigned id = blockIdx.x * waves + wave;
+    Item cur{0, 0, 0, 0};
+    double pos0 = 0.0;
+    if (id < p.items) {
+        cur = locate(id);
+        pos0 = pos_of(cur);
+        if (cur.r0 + sub < cur.r_end) load(cur, cur.r0 + sub);
+    }
+    while (id < p.items) {
         for (int pr = lane; pr < chunks * W; pr += 64) {
             float2 cs = make_float2(1.f, 0.f);
             if (pr < R2) {
-                int a = 0;
-#pragma unroll
-                for (int i = 0; i < ROT_MAX_AXES - 1; ++i) a += (i + 1 < p.n_axes && pr >= p.axis_end[i]);
-                cs = cos_sin(load_pos(p, b, n, a), p.freq[pr]);
+                cs = pr == lane ? cos_sin(pos0, freq0) : cos_sin(load_pos(p, cur.b, cur.n, axis_of(pr)), p.freq[pr]);
                 cs.y *= p.sign;
             }
             table[pr] = cs;
+        }
+        // the next item's position and, behind this one's last heads, its first are on their way while this one is worked on
+        const unsigned next_id = id + gridDim.x * waves;
+        Item next{0, 0, 0, 0};
+        if (next_id < p.items) {
+            next = locate(next_id);
+            pos0 = pos_of(next);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -166,18 +225,20 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();  // the table is read before the next item overwrites it
 
-        // all lanes of the wave walk the same number of steps: the shuffles below need every lane of a head
-        const int steps = (r_end - share * p.rows_per_item + row_step - 1) >> (6 - lp_log2);
-        for (int it = 0; it < steps; ++it, r += row_step) {
-            const bool row_on = r < r_end;
+        // all lanes of the wave walk the same number of steps: the sums below need every lane of a head
+        for (int r00 = cur.r0; r00 < cur.r_end; r00 += row_step) {
+            const int r = r00 + sub;
+            const bool row_on = r < cur.r_end;
+            const int seg = r >= p.heads[0];
             float a[NC][2 * W], g[NC][2 * W];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 to_f32<T, W>(v0[c], a[c]); to_f32<T, W>(v1[c], a[c] + W);
                 if constexpr (BWD) { to_f32<T, W>(g0[c], g[c]); to_f32<T, W>(g1[c], g[c] + W); }
             }
-            if (it + 1 < steps && r + row_step < r_end) load(r + row_step);
-            const int seg = r >= p.heads[0];
+            if (r00 + row_step < cur.r_end) {
+                if (r + row_step < cur.r_end) load(cur, r + row_step);
+            } else if (next.r0 + sub < next.r_end) load(next, next.r0 + sub);
 
             // index of a pair's two channels among the lane's 2W
             auto turn = [&](float *y, int c) __attribute__((always_inline)) {
@@ -195,36 +256,47 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
                     for (int i = 0; i < 2 * W; ++i) ss += a[c][i] * a[c][i];
-                float gx = 0.f;
+                float w[NC][2 * W];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const float *ws = weights + (seg ? wpad : 0);
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        w[c][i] = ws[on0[c] ? e0[c] + i : 0];
+                        w[c][W + i] = ws[on1[c] ? e1[c] + i : 0];
+                    }
+                }
                 if constexpr (BWD) {
+                    float gx = 0.f;
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
                         turn(g[c], c);
 #pragma unroll
-                        for (int i = 0; i < 2 * W; ++i) gx += g[c][i] * (seg ? w[1][c][i] : w[0][c][i]) * a[c][i];
+                        for (int i = 0; i < 2 * W; ++i) gx += g[c][i] * w[c][i] * a[c][i];
                     }
-                }
-                for (int m = 1; m < LP; m <<= 1) {
-                    ss += __shfl_xor(ss, m);
-                    if constexpr (BWD) gx += __shfl_xor(gx, m);
-                }
-                const float rho = 1.f / sqrtf(ss * inv_d + p.eps);
-                const float k = gx * inv_d * rho * rho;  // mean(g w xh) rho^-1 ... times xh = x rho below
+                    ss = head_sum(ss, lp_log2);
+                    gx = head_sum(gx, lp_log2);
+                    const float rho = inverse_root(ss * inv_d + p.eps);
+                    const float k = gx * inv_d * rho * rho;  // mean(g w xh) rho: xh mean(g w xh) = x k
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+                    for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int i = 0; i < 2 * W; ++i) {
-                        const float wi = seg ? w[1][c][i] : w[0][c][i];
-                        if constexpr (BWD) {
+                        for (int i = 0; i < 2 * W; ++i) {
                             const float gi = row_on ? g[c][i] * (a[c][i] * rho) : 0.f;
                             dw[0][c][i] += seg ? 0.f : gi;
                             dw[1][c][i] += seg ? gi : 0.f;
-                            a[c][i] = rho * (g[c][i] * wi - a[c][i] * k);
-                        } else a[c][i] = a[c][i] * rho * wi;
-                    }
+                            a[c][i] = rho * (g[c][i] * w[c][i] - a[c][i] * k);
+                        }
+                } else {
+                    const float rho = inverse_root(head_sum(ss, lp_log2) * inv_d + p.eps);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int i = 0; i < 2 * W; ++i) a[c][i] = a[c][i] * rho * w[c][i];
+                }
             }
             if (row_on) {
-                T *dst = offset(p.out, r);
+                T *dst = at(p.out, cur, r);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     if constexpr (!BWD) turn(a[c], c);
@@ -233,12 +305,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
                 }
             }
         }
+        id = next_id;
+        cur = next;
     }
 
     if constexpr (BWD) {
         // weight gradients: the wave's heads by shuffles, the workgroup's waves through LDS in wave order, one row of partials per
         // workgroup (summed in order by rotary_dw_kernel: the same bits every time)
-        float *red = reinterpret_cast<float *>(table_all);  // [waves][2][D]
+        float *red = reinterpret_cast<float *>(smem);  // [waves][2][D]
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -266,8 +340,14 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float *part, int 
     __shared__ float red[64][17];
     const int col = blockIdx.x * 16 + (threadIdx.x & 15), grp = threadIdx.x >> 4;
     float t = 0.f;
-    if (col < 2 * D)
-        for (int k = grp; k < blocks; k += 64) t += part[(size_t)k * 2 * D + col];
+    if (col < 2 * D) {
+        static_assert(ROT_BWD_BLOCKS % 64 == 0, "");
+        float v[ROT_BWD_BLOCKS / 64];  // all on their way at once
+#pragma unroll
+        for (int k = 0; k < ROT_BWD_BLOCKS / 64; ++k) v[k] = grp + 64 * k < blocks ? part[(size_t)(grp + 64 * k) * 2 * D + col] : 0.f;
+#pragma unroll
+        for (int k = 0; k < ROT_BWD_BLOCKS / 64; ++k) t += v[k];
+    }
     red[grp][threadIdx.x & 15] = t;
     __syncthreads();
     if (grp == 0 && col < 2 * D) {
@@ -284,13 +364,14 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float *part, int 
 template <typename T, int W, int NC, bool HALVES>
 int launch_mode(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks, void *dw0, void *dw1, hipStream_t s) {
     const int chunks = ((p.D + 1) / 2 + W - 1) / W;
-    size_t lds = (size_t)4 * chunks * W * sizeof(float2);
+    const int waves = mode == ROT_NORM_BWD ? ROT_BWD_THREADS / 64 : 4;
+    size_t lds = (size_t)waves * chunks * W * sizeof(float2) + (mode == ROT_PLAIN ? 0 : 2 * ((p.D + 3) & ~3) * sizeof(float));
     switch (mode) {
         case ROT_PLAIN: rotary_kernel<T, W, NC, HALVES, ROT_PLAIN><<<blocks, 256, lds, s>>>(p, lp_log2); break;
         case ROT_NORM: rotary_kernel<T, W, NC, HALVES, ROT_NORM><<<blocks, 256, lds, s>>>(p, lp_log2); break;
         case ROT_NORM_BWD:
-            if (lds < (size_t)4 * 2 * p.D * sizeof(float)) lds = (size_t)4 * 2 * p.D * sizeof(float);
-            rotary_kernel<T, W, NC, HALVES, ROT_NORM_BWD><<<blocks, 256, lds, s>>>(p, lp_log2);
+            if (lds < (size_t)waves * 2 * p.D * sizeof(float)) lds = (size_t)waves * 2 * p.D * sizeof(float);
+            if constexpr (W * sizeof(T) <= 8 || sizeof(T) == 4) rotary_kernel<T, W, NC, HALVES, ROT_NORM_BWD><<<blocks, ROT_BWD_THREADS, lds, s>>>(p, lp_log2);
             GD_HIP(hipGetLastError());
             rotary_dw_kernel<T><<<(2 * p.D + 15) / 16, 1024, 0, s>>>(p.dw_part, blocks, p.D, dw0, dw1, p.w_f32);
             break;
@@ -321,7 +402,8 @@ template <typename T>
 int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStream_t s) {
     constexpr int WV = 16 / sizeof(T);
     const bool bwd = mode == ROT_NORM_BWD;
-    const int W = vec_ok(p, WV, sizeof(T), bwd) ? WV : vec_ok(p, WV / 2, sizeof(T), bwd) ? WV / 2 : 1;
+    const bool narrow = sizeof(T) == 2 && bwd;  // half the registers, twice the waves: 69 us against 87 for 16 + 4 heads of 128 channels at 16382 tokens
+    const int W = !narrow && vec_ok(p, WV, sizeof(T), bwd) ? WV : vec_ok(p, WV / 2, sizeof(T), bwd) ? WV / 2 : 1;
     const int chunks = ((p.D + 1) / 2 + W - 1) / W;
     int lp_log2 = 0;
     while (lp_log2 < 6 && (1 << lp_log2) < chunks) ++lp_log2;
@@ -341,7 +423,8 @@ int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStrea
     p.rows_per_item = (int)((steps + shares - 1) / shares) * row_step;
     p.items_per_token = (rows + p.rows_per_item - 1) / p.rows_per_item;
     p.items = (unsigned)(tokens * p.items_per_token);  // < 2^31: shares are taken only where tokens are few
-    unsigned blocks = (p.items + 3) / 4;
+    const unsigned per_block = bwd ? ROT_BWD_THREADS / 64 : 4;
+    unsigned blocks = (p.items + per_block - 1) / per_block;
     if (blocks > (unsigned)max_blocks) blocks = max_blocks;
     if (W == WV && chunks <= 64) return launch_pairs<T, WV, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
     if (W == WV / 2 && W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);

@@ -8,7 +8,8 @@ namespace gd {
 
 constexpr int ROT_MAX_AXES = 4;
 constexpr int ROT_MAX_HEAD_DIM = 512;
-constexpr int ROT_BWD_BLOCKS = 1024;  // partial rows of the weight gradients
+constexpr int ROT_BWD_BLOCKS = 512;  // partial rows of the weight gradients
+constexpr int ROT_BWD_THREADS = 512;
 
 // one (B, N, heads, D) tensor: strides in elements, channels adjacent
 struct HeadsView {
