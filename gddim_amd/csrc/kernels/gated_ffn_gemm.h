@@ -198,7 +198,7 @@ struct Operand {
     __device__ static __forceinline__ int piece_of(int i, int wave, int lane) { return lane % CPR ^ swizzle(row_of(i % PERIOD, wave, lane)); }
     __device__ static __forceinline__ int swizzle(int r) {
         if constexpr (KC) return kc_swizzle(r);
-        else if constexpr (ES == 2) return 4 * (r & 3);
+        else if constexpr (ES == 2) return 4 * (r & 3);  // four k rows of 64 bytes on different banks
         else return 8 * ((r >> 2) & 1);
     }
     // gated B tiles: rows of gate and up alternate in blocks of 32, so that a wave's 64 columns hold both of its 32
