@@ -74,6 +74,7 @@ class FfnDesc(ctypes.Structure):
         ("in_", ctypes.c_int),
         ("hidden", ctypes.c_int),
         ("out", ctypes.c_int),
+        ("unaligned", ctypes.c_int),
         ("ld_x", ctypes.c_longlong),
         ("ld_w_in", ctypes.c_longlong),
         ("ld_w_down", ctypes.c_longlong),

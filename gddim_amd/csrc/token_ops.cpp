@@ -193,7 +193,7 @@ FfnLaunches ffn_launches(const gd_ffn_desc *d, const void *x, const void *wg, co
         Wd{wd, d->out, d->hidden, d->ld_w_down}, H{hidden, d->rows, d->hidden, d->hidden}, DY{dy, d->rows, d->out, ld_dy},
         DG{dgate, d->rows, d->hidden, d->hidden}, DU{dup, d->rows, d->hidden, d->hidden};
     FfnLaunches f{};
-    for (auto &l : f.l) { l.problems = 1; l.direct = 1; l.act = d->act; }
+    for (auto &l : f.l) { l.problems = 1; l.direct = !d->unaligned; l.act = d->act; }
     const Matrix w_in[2] = {Wg, Wu}, d_in[2] = {DG, DU};
     f.l[GEMM_GATE_UP].q[0] = problem(&X, true, w_in, true, 1, true, es, &f.l[GEMM_GATE_UP].direct);
     f.l[GEMM_DOWN].q[0] = problem(&H, true, &Wd, true, 1, false, es, &f.l[GEMM_DOWN].direct);
@@ -209,17 +209,26 @@ FfnLaunches ffn_launches(const gd_ffn_desc *d, const void *x, const void *wg, co
 
 long long align_up(long long n) { return (n + 255) / 256 * 256; }
 
-// floats of partial sums any of the given launches may need, whatever the alignment of the tensors turns out to be
+// the same as the workspace's size is computed from: aligned tensors, dense rows of dy
+FfnLaunches ffn_sizing(const gd_ffn_desc *d) {
+    return ffn_launches(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, d->out, nullptr, nullptr);
+}
+
+// floats of partial sums that the given launches need
 long long partial_floats(FfnLaunches f, int dtype, int first, int last) {
     long long most = 0;
-    for (int k = first; k <= last; ++k)
-        for (int direct = 0; direct < 2; ++direct) {
-            GemmLaunch l = f.l[k];
-            l.direct = direct;
-            const long long n = plan_gemm(l, dtype, (GemmKind)k);
-            if (n > most) most = n;
-        }
+    for (int k = first; k <= last; ++k) {
+        const long long n = plan_gemm(f.l[k], dtype, (GemmKind)k);
+        if (n > most) most = n;
+    }
     return most;
+}
+
+int check_as_sized(const FfnLaunches &f, const gd_ffn_desc *d, int first, int last, const char *who) {
+    const FfnLaunches sized = ffn_sizing(d);
+    for (int k = first; k <= last; ++k)
+        GD_CHECK(f.l[k].direct == sized.l[k].direct, "%s: a tensor does not start (or rows of dy are not apart by) a multiple of 16 bytes: set unaligned", who);
+    return 0;
 }
 
 }  // namespace
@@ -228,7 +237,7 @@ extern "C" {
 
 long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward) {
     if (check_ffn(d, "gated_ffn_workspace")) return -1;
-    const FfnLaunches f = ffn_launches(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, d->out, nullptr, nullptr);
+    const FfnLaunches f = ffn_sizing(d);
     if (!backward) return partial_floats(f, d->dtype, GEMM_GATE_UP, GEMM_DOWN) * (long long)sizeof(float);
     const long long grad = align_up((long long)d->rows * d->hidden * (long long)elem_size(d->dtype));
     return 2 * grad + partial_floats(f, d->dtype, GEMM_DHIDDEN, GEMM_DW) * (long long)sizeof(float);
@@ -245,6 +254,7 @@ int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const 
     GD_CHECK((uintptr_t)workspace_dev % 16 == 0, "%s: workspace not aligned to 16 bytes", who);
     GD_CHECK(workspace_dev || gd_gated_ffn_workspace(d, 0) == 0, "%s: null workspace", who);
     FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden_dev, nullptr, d->out, nullptr, nullptr);
+    GD_TRY(check_as_sized(f, d, GEMM_GATE_UP, GEMM_DOWN, who));
     GemmLaunch &g = f.l[GEMM_GATE_UP], &o = f.l[GEMM_DOWN];
     g.q[0].out[0] = hidden_dev; g.q[0].out[1] = gate_dev; g.q[0].out[2] = up_dev;
     o.q[0].out[0] = y;
@@ -266,6 +276,7 @@ int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy,
     void *dgate = ws, *dup = ws ? ws + grad : nullptr;
     float *partial = reinterpret_cast<float *>(ws ? ws + 2 * grad : nullptr);
     FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden, dy, ld_dy, dgate, dup);
+    GD_TRY(check_as_sized(f, d, empty ? GEMM_DW : GEMM_DHIDDEN, GEMM_DW, who));
     hipStream_t s = (hipStream_t)stream;
     if (!empty) {
         GemmProblem &h = f.l[GEMM_DHIDDEN].q[0];

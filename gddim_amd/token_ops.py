@@ -262,22 +262,22 @@ def _check_ffn(x, w_gate, w_up, w_down, act):
     rows = x.shape[0]
     if rows > 1 << 30 or gs[0] > 1 << 30 or gs[1] > 1 << 30 or ds[0] > 1 << 30:
         raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (rows, gs[1], gs[0], ds[0]))
-    return x, w_gate, w_up, w_down, FfnDesc(code, kind, rows, gs[1], gs[0], ds[0], x.stride(0), ld, w_down.stride(0))
+    unaligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr() | w_down.data_ptr()) & 15 != 0
+    return x, w_gate, w_up, w_down, FfnDesc(code, kind, rows, gs[1], gs[0], ds[0], unaligned, x.stride(0), ld, w_down.stride(0))
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(dtype, rows, in_, hidden, out, backward, device):
+def _workspace_bytes(backward, device, *desc):
     """gd_gated_ffn_workspace of these sizes on this device (its compute units count)"""
-    desc = FfnDesc(dtype, 0, rows, in_, hidden, out, in_, in_, hidden)
     with _torch()[0].cuda.device(device):
-        n = _abi.lib().gd_gated_ffn_workspace(desc, backward)
+        n = _abi.lib().gd_gated_ffn_workspace(FfnDesc(*desc), backward)
     if n < 0:
         check(1)
     return n
 
 
 def _workspace(x, d, backward):
-    n = _workspace_bytes(d.dtype, d.rows, d.in_, d.hidden, d.out, backward, x.get_device())
+    n = _workspace_bytes(backward, x.get_device(), d.dtype, 0, d.rows, d.in_, d.hidden, d.out, d.unaligned, d.ld_x, d.ld_w_in, d.ld_w_down)
     return x.new_empty(n, dtype=_torch()[0].uint8) if n else None
 
 
@@ -316,6 +316,8 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
             raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
     dy = _rows(dy, O)
     gate, up, hidden = saved
+    if (dy.data_ptr() | gate.data_ptr() | up.data_ptr() | hidden.data_ptr()) & 15 or (dy.stride(0) != O and dy.stride(0) * dy.element_size() % 16):
+        desc.unaligned = 1
     dx, dwg, dwu, dwd = x.new_empty((M, D)), x.new_empty((F, D)), x.new_empty((F, D)), x.new_empty((O, F))
     ws = _workspace(x, desc, 1)
     _call(x, _abi.lib().gd_gated_ffn_backward, desc, dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),

@@ -394,13 +394,16 @@ int gd_qk_norm_rotary_backward(const gd_rotary_desc *d, const gd_heads *dq_out, 
                                const gd_heads *dq, const gd_heads *dk, int heads_q, int heads_k, const void *w_q, const void *w_k, int w_f32,
                                float eps, void *workspace_dev, void *dw_q, void *dw_k, void *stream);
 /* Gated feed-forward block on `rows` tokens:  y = (act(x w_gate^T) (.) (x w_up^T)) w_down^T,  x (rows, in), w_gate and w_up (hidden, in),
- * w_down (out, hidden), y (rows, out); act: GD_ACT_*.  Leading dimensions in elements (w_gate and w_up share one). */
+ * w_down (out, hidden), y (rows, out); act: GD_ACT_*.  Leading dimensions in elements (w_gate and w_up share one).  unaligned == 0 says that every
+ * tensor of the calls starts at a multiple of 16 bytes and that the rows of dy are `out` or a multiple of 16 bytes apart (checked); != 0 takes any tensor, and
+ * sizes the workspace for that. */
 typedef struct gd_ffn_desc {
     int dtype, act;
     int rows, in, hidden, out;
+    int unaligned;
     long long ld_x, ld_w_in, ld_w_down;
 } gd_ffn_desc;
-/* hidden_dev (rows, hidden) receives act(gate) (.) up; gate_dev and up_dev (rows, hidden) the projections in fp32 whatever the tensors' type, or both
+/* hidden_dev (rows, hidden) receives act(gate) (.) up in the tensors' type (fp16: up to 65504); gate_dev and up_dev (rows, hidden) the projections in fp32 whatever the tensors' type, or both
  * null: what the backward call needs of a training step.  workspace_dev: gd_gated_ffn_workspace(d, 0) bytes (may be 0), 16-byte aligned. */
 long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward);
 int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, float *gate_dev, float *up_dev,

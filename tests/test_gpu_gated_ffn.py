@@ -80,6 +80,114 @@ def test_tiles_that_fill_the_chip(dev, size, typ):
 
 
 @pytest.mark.parametrize("typ", ["bf16", "f32"])
+@pytest.mark.parametrize("size", [(8200, 64, 2600, 64), (8200, 72, 2600, 72), (8200, 200, 1304, 1304), (8200, 65, 1301, 67), (16000, 24, 2056, 24)], ids=str)
+def test_more_tiles_than_workgroups(dev, size, typ):
+    """a workgroup walks several tiles, of one stage of k and of more"""
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ], 2)
+    want = ref.gated_ffn(x, wg, wu, wd, "gelu_tanh", TYPES[typ], dy)
+    got = _run(x, wg, wu, wd, dy, "gelu_tanh")
+    for g, w, what in zip(got, want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+    for a, b in zip(got, _run(x, wg, wu, wd, dy, "gelu_tanh")):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [(1, 8, 8, 8), (1, 520, 4104, 1032), (4, 1024, 40, 8), (16, 264, 4104, 2056), (17, 64, 2064, 1032), (48, 72, 136, 24), (64, 1000, 1024, 4104),
+                                  (100, 64, 136, 72), (256, 64, 200, 64), (255, 128, 352, 128)], ids=str)
+def test_few_rows(dev, size, typ):
+    from gddim_amd import ops
+    x, wg, wu, wd, _ = _inputs(dev, *size, TYPES[typ], 4)
+    for kind in ("silu", "gelu"):
+        y, saved = ops.gated_ffn(x, wg, wu, wd, act=kind, save=True)
+        _check(y, ref.gated_ffn(x, wg, wu, wd, kind, TYPES[typ]), "y")
+        gate, up = ref.product(ref.V(x.double()), ref.V(wg.double())), ref.product(ref.V(x.double()), ref.V(wu.double()))
+        _check(saved[0], gate, "gate")
+        _check(saved[1], up, "up")
+        _check(saved[2], (ref.act(gate, kind)[0] * up).rounded(TYPES[typ]), "hidden")
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+@pytest.mark.parametrize("size", [(1, 64, 72, 40), (65, 72, 130, 66), (300, 33, 17, 9), (4100, 72, 520, 64)], ids=str)
+def test_nothing_is_written_beside_the_results(dev, native_lib, size, typ):
+    """the C entry points on buffers between guard values"""
+    from gddim_amd._abi import FfnDesc
+    M, D, F, O = size
+    dtype = TYPES[typ]
+    x, wg, wu, wd, dy = _inputs(dev, *size, dtype, 9)
+    pad = 1024
+
+    def guarded(rows, cols, dt=dtype):
+        buf = torch.full((rows * cols + 2 * pad,), 12345.0, dtype=dt, device=dev)
+        return buf, buf[pad:pad + rows * cols].view(rows, cols)
+
+    for unaligned in (0, 1):
+        d = FfnDesc(0 if typ == "f32" else 1, 0, M, D, F, O, unaligned, D, D, F)
+        s = torch.cuda.current_stream().cuda_stream
+        bufs = [guarded(M, F, torch.float32), guarded(M, F, torch.float32), guarded(M, F), guarded(M, O), guarded(M, D), guarded(F, D), guarded(F, D), guarded(O, F)]
+        ws = [guarded(1, max(4, native_lib.gd_gated_ffn_workspace(d, b) // 4), torch.float32) for b in (0, 1)]
+        p = [v.data_ptr() for _, v in bufs]
+        assert native_lib.gd_gated_ffn(d, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p[0], p[1], p[2], p[3], ws[0][1].data_ptr(), s) == 0
+        assert native_lib.gd_gated_ffn_backward(d, dy.data_ptr(), O, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p[0], p[1], p[2], p[4], p[5], p[6], p[7],
+                                                ws[1][1].data_ptr(), s) == 0
+        torch.cuda.synchronize()
+        for buf, v in bufs + ws:
+            assert (buf[:pad] == buf[0]).all() and (buf[-pad:] == buf[0]).all() and buf[0] == torch.tensor(12345.0, dtype=buf.dtype)
+        want = ref.gated_ffn(x, wg, wu, wd, "silu", dtype, dy)
+        for i, w in zip((3, 4, 5, 6, 7), want):
+            _check(bufs[i][1], w, "result %d" % i)
+
+
+def test_offsets_past_32_bits(dev):
+    """hidden rows past 2^31 elements, first and last rows checked, all others zero"""
+    from gddim_amd import ops
+    M, D, F, O = 540000, 64, 4096, 64
+    rows = torch.tensor([0, 1, 255, 256, 300000, M - 2, M - 1], device=dev)
+    x, wg, wu, wd, dy = _inputs(dev, len(rows), D, F, O, torch.bfloat16, 10)
+    want = ref.gated_ffn(x, wg, wu, wd, "silu", torch.bfloat16, dy)
+    big_x, big_dy = torch.zeros(M, D, dtype=x.dtype, device=dev), torch.zeros(M, O, dtype=x.dtype, device=dev)
+    big_x[rows], big_dy[rows] = x, dy
+    y, saved = ops.gated_ffn(big_x, wg, wu, wd, save=True)
+    assert saved[0].numel() > 1 << 31
+    dx, *dw = ops.gated_ffn_backward(big_dy, big_x, wg, wu, wd, saved)
+    _check(y[rows], want[0], "y")
+    _check(dx[rows], want[1], "dx")
+    for g, w, what in zip(dw, want[2:], ("dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+    others = torch.ones(M, dtype=torch.bool, device=dev)
+    others[rows] = False
+    assert (y[others] == 0).all() and (dx[others] == 0).all()
+
+
+def test_two_streams_at_once(dev):
+    a, b = _inputs(dev, 700, 256, 688, 256, torch.bfloat16, 11), _inputs(dev, 700, 256, 688, 256, torch.bfloat16, 12)
+    want = [_run(*t, "silu") for t in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(_run(*t, "silu"))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(p, q) for p, q in zip(run, want[i]))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_tensors_of_another_device():
+    from gddim_amd import ops
+    other = torch.device("cuda", 1)
+    x, wg, wu, wd, dy = _inputs(other, 70, 64, 136, 64, torch.bfloat16)
+    with torch.cuda.device(0):
+        got = _run(x, wg, wu, wd, dy, "silu")
+    for g, w in zip(got, ref.gated_ffn(x, wg, wu, wd, "silu", torch.bfloat16, dy)):
+        assert g.device == other
+        _check(g, w, "on the second device")
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
 def test_strides_and_batches(dev, typ):
     """rows and weights seen through larger matrices, both projections packed, channels not adjacent, batches of any rank, rows off any alignment"""
     from gddim_amd import ops

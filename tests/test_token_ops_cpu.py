@@ -90,7 +90,7 @@ def test_float64_forms_against_autograd(paired):
 
 def _ffn(**kw):
     from gddim_amd._abi import FfnDesc
-    d = dict(dtype=1, act=0, rows=4, in_=8, hidden=16, out=8, ld_x=8, ld_w_in=8, ld_w_down=16)
+    d = dict(dtype=1, act=0, rows=4, in_=8, hidden=16, out=8, unaligned=0, ld_x=8, ld_w_in=8, ld_w_down=16)
     d.update(kw)
     return FfnDesc(**d)
 
@@ -116,6 +116,10 @@ def test_c_gated_ffn_refuses_arguments(native_lib):
     assert native_lib.gd_gated_ffn(d, 64, 64, 64, 64, None, None, 64, 64, 72, None) != 0  # workspace off its alignment
     assert native_lib.gd_gated_ffn_backward(d, 64, 7, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None) != 0
     assert native_lib.gd_gated_ffn_backward(d, 64, 8, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None, None) != 0
+    assert native_lib.gd_gated_ffn(d, 72, 64, 64, 64, None, None, 64, 64, 64, None) != 0  # a tensor off its alignment and not said so
+    assert b"unaligned" in native_lib.gd_last_error()
+    assert native_lib.gd_gated_ffn_backward(d, 64, 9, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, None) != 0  # ... rows of dy
+    assert b"unaligned" in native_lib.gd_last_error()
     assert native_lib.gd_gated_ffn(_ffn(rows=0), None, 64, 64, 64, None, None, None, None, None, None) == 0  # no rows: nothing is launched
     assert native_lib.gd_gated_ffn_workspace(d, 1) >= 2 * 4 * 16 * 2
 
