@@ -87,9 +87,7 @@ _LL = ctypes.c_longlong
 _F = ctypes.c_float
 _D = ctypes.c_double
 _SZ = ctypes.c_size_t
-_H = ctypes.POINTER(Heads)
-_RD = ctypes.POINTER(RotaryDesc)
-_FD = ctypes.POINTER(FfnDesc)
+_H = _RD = _FD = ctypes.c_void_p  # gd_heads, gd_rotary_desc, gd_ffn_desc: ctypes.byref(structure) or its bytes
 
 # name -> (restype, argtypes); every symbol include/gddim_amd.h declares
 SIGNATURES = {

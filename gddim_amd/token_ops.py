@@ -4,13 +4,15 @@ pass, the gated feed-forward block (include/gddim_amd.h, "token operators").
 Tensors are float32, bfloat16 or float16 and stay in their type; work is queued on the current stream of the tensors' device, nothing
 synchronises, and every call can be captured into a graph.  The operators record no autograd graph: gradients come from the *_backward calls, and a
 tensor that requires grad is refused while grad mode is on.  No reference counterpart."""
-import ctypes
 import functools
 import math
+import struct
 
 from . import _abi
-from ._abi import FfnDesc, GddimError, Heads, RotaryDesc, check
+from ._abi import GddimError, check
 
+# gd_rotary_desc, gd_heads and gd_ffn_desc as bytes: packed in a third of the time that filling a ctypes structure takes
+_ROTARY, _HEADS, _FFN = struct.Struct("@11iP3qP"), struct.Struct("@P3q"), struct.Struct("@7i3q")
 _TORCH = None
 
 
@@ -84,15 +86,14 @@ class RotaryAxes:
         device = torch.device("cuda") if device is None else torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.frequencies = torch.as_tensor(frequencies, dtype=torch.float64).detach().to(device).contiguous()
+        self.frequencies = torch.as_tensor(frequencies, dtype=torch.float64).detach().to(device).clone(memory_format=torch.contiguous_format)
         if tuple(self.frequencies.shape) != (sum(self.sections) // 2,):
             raise GddimError("RotaryAxes: frequencies of shape %s, expected (%d,)" % (tuple(self.frequencies.shape), sum(self.sections) // 2))
         self.device = device
         self._rotated = sum(self.sections)
         self._index = device.index if device.type == "cuda" else -1
         self._halves = int(paired == "halves")
-        self._table = self.frequencies.data_ptr()
-        self._section = (ctypes.c_int * _abi.GD_MAX_AXES)(*self.sections)
+        self._section = self.sections + (0,) * (_abi.GD_MAX_AXES - len(self.sections))
 
 
 def _heads(t):
@@ -101,7 +102,13 @@ def _heads(t):
     if s[3] != 1 and t.shape[3] > 1:
         t = t.contiguous()
         s = t.stride()
-    return t, Heads(t.data_ptr(), s[0], s[1], s[2])
+    return t, _HEADS.pack(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _dense_heads(t):
+    """the view of an output of _new"""
+    s = t.stride()
+    return _HEADS.pack(t.data_ptr(), s[0], s[1], s[2])
 
 
 def _check_heads(t, name, like=None, like_name=None):
@@ -150,7 +157,7 @@ def _rotary_desc(x, pos, axes):
         raise GddimError("sections %r of %d channels exceed the head's %d" % (axes.sections, axes._rotated, D))
     if B * N >= 1 << 31:
         raise GddimError("%d x %d tokens do not fit 31 bits" % (B, N))
-    return RotaryDesc(types[x.dtype], B, N, D, A, axes._section, axes._halves, kind, pos.data_ptr(), sb, sn, sa, axes._table)
+    return _ROTARY.pack(types[x.dtype], B, N, D, A, *axes._section, axes._halves, kind, pos.data_ptr(), sb, sn, sa, axes.frequencies.data_ptr())
 
 
 def rotary(x, pos, axes, inverse=False):
@@ -161,9 +168,8 @@ def rotary(x, pos, axes, inverse=False):
     _check_heads(x, "x")
     desc = _rotary_desc(x, pos, axes)
     out = _new(x)
-    x, xv = _heads(x)
-    _, ov = _heads(out)
-    _call(x, _abi.lib().gd_rotary, desc, xv, ov, x.shape[2], int(bool(inverse)))
+    x, view = _heads(x)
+    _call(x, _abi.lib().gd_rotary, desc, view, _dense_heads(out), x.shape[2], int(bool(inverse)))
     return out
 
 
@@ -202,7 +208,7 @@ def qk_norm_rotary(q, k, weight_q, weight_k, pos, axes, eps=1e-6):
     desc = _rotary_desc(q, pos, axes)
     qo, ko = _new(q), _new(k)
     (q, qv), (k, kv) = _heads(q), _heads(k)
-    _call(q, _abi.lib().gd_qk_norm_rotary, desc, qv, kv, _heads(qo)[1], _heads(ko)[1], q.shape[2], k.shape[2], p_q, p_k, w_f32, eps)
+    _call(q, _abi.lib().gd_qk_norm_rotary, desc, qv, kv, _dense_heads(qo), _dense_heads(ko), q.shape[2], k.shape[2], p_q, p_k, w_f32, eps)
     return qo, ko
 
 
@@ -221,7 +227,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, weight_q, weight_k, pos, axes,
     (q, qv), (k, kv), (dq_out, gqv), (dk_out, gkv) = _heads(q), _heads(k), _heads(dq_out), _heads(dk_out)
     lib = _abi.lib()
     ws = q.new_empty(lib.gd_qk_norm_rotary_backward_workspace(q.shape[3]), dtype=torch.uint8)
-    _call(q, lib.gd_qk_norm_rotary_backward, desc, gqv, gkv, qv, kv, _heads(dq)[1], _heads(dk)[1], q.shape[2], k.shape[2], p_q, p_k, w_f32, eps, ws.data_ptr(),
+    _call(q, lib.gd_qk_norm_rotary_backward, desc, gqv, gkv, qv, kv, _dense_heads(dq), _dense_heads(dk), q.shape[2], k.shape[2], p_q, p_k, w_f32, eps, ws.data_ptr(),
           dwq.data_ptr() if dwq is not None else None, dwk.data_ptr() if dwk is not None else None)
     return dq, dk, dwq, dwk
 
@@ -242,7 +248,7 @@ def _rows(t, columns):
 
 
 def _check_ffn(x, w_gate, w_up, w_down, act):
-    """(x as a matrix, the weights with adjacent columns, the call's description)"""
+    """(x as a matrix, the weights with adjacent columns, the fields of gd_ffn_desc)"""
     _on_gpu(x, "x")
     code, kind = _torch()[1].get(x.dtype), _ACTS.get(act)
     if kind is None:
@@ -262,65 +268,70 @@ def _check_ffn(x, w_gate, w_up, w_down, act):
     rows = x.shape[0]
     if rows > 1 << 30 or gs[0] > 1 << 30 or gs[1] > 1 << 30 or ds[0] > 1 << 30:
         raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (rows, gs[1], gs[0], ds[0]))
-    unaligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr() | w_down.data_ptr()) & 15 != 0
-    return x, w_gate, w_up, w_down, FfnDesc(code, kind, rows, gs[1], gs[0], ds[0], unaligned, x.stride(0), ld, w_down.stride(0))
+    unaligned = int((x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr() | w_down.data_ptr()) & 15 != 0)
+    return x, w_gate, w_up, w_down, (code, kind, rows, gs[1], gs[0], ds[0], unaligned, x.stride(0), ld, w_down.stride(0))
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(backward, device, *desc):
+def _workspace_bytes(fields, backward, device):
     """gd_gated_ffn_workspace of these sizes on this device (its compute units count)"""
     with _torch()[0].cuda.device(device):
-        n = _abi.lib().gd_gated_ffn_workspace(FfnDesc(*desc), backward)
+        n = _abi.lib().gd_gated_ffn_workspace(_FFN.pack(*fields), backward)
     if n < 0:
         check(1)
     return n
 
 
-def _workspace(x, d, backward):
-    n = _workspace_bytes(backward, x.get_device(), d.dtype, 0, d.rows, d.in_, d.hidden, d.out, d.unaligned, d.ld_x, d.ld_w_in, d.ld_w_down)
-    return x.new_empty(n, dtype=_torch()[0].uint8) if n else None
+def _workspace(x, fields, backward):
+    """(tensor or None, its address or None)"""
+    n = _workspace_bytes(fields, backward, x.get_device())
+    if not n:
+        return None, None
+    t = x.new_empty(n, dtype=_torch()[0].uint8)
+    return t, t.data_ptr()
 
 
 def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
     """Gated feed-forward block (act(x w_gate^T) * (x w_up^T)) w_down^T: x (..., in), weights as torch.nn.Linear keeps them -- w_gate and w_up
     (hidden, in), w_down (out, hidden) -- act 'silu', 'gelu' or 'gelu_tanh'.  Returns y (..., out); with save=True (y, saved), saved for
     gated_ffn_backward (the two projections in float32 and their product).  Both projections, the activation and the product are one kernel."""
-    shape = x.shape if isinstance(x, _torch()[0].Tensor) else ()
-    x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
-    y, hidden, ws = x.new_empty((desc.rows, desc.out)), x.new_empty((desc.rows, desc.hidden)), _workspace(x, desc, 0)
-    gate, up = (x.new_empty((desc.rows, desc.hidden), dtype=_torch()[0].float32) for _ in range(2)) if save else (None, None)
-    _call(x, _abi.lib().gd_gated_ffn, desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
-          up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws.data_ptr() if ws is not None else None)
-    if len(shape) != 2:
-        y = y.view(*shape[:-1], desc.out)
+    x_in = x
+    x, w_gate, w_up, w_down, fields = _check_ffn(x, w_gate, w_up, w_down, act)
+    rows, F, O = fields[2], fields[4], fields[5]
+    y, hidden = x.new_empty((rows, O)), x.new_empty((rows, F))
+    ws, ws_at = _workspace(x, fields, 0)
+    if save:
+        gate, up = (x.new_empty((rows, F), dtype=_torch()[0].float32) for _ in range(2))
+    _call(x, _abi.lib().gd_gated_ffn, _FFN.pack(*fields), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), gate.data_ptr() if save else None,
+          up.data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), ws_at)
+    if x_in.dim() != 2:
+        y = y.view(*x_in.shape[:-1], O)
     return (y, (gate, up, hidden)) if save else y
 
 
 def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
     """Gradients (dx, dw_gate, dw_up, dw_down) of gated_ffn from that of its result and what the call with save=True kept (left as it was).  The
     same bits every time."""
-    torch = _torch()[0]
-    shape = x.shape if isinstance(x, torch.Tensor) else ()
-    x, w_gate, w_up, w_down, desc = _check_ffn(x, w_gate, w_up, w_down, act)
-    M, D, F, O = x.shape[0], x.shape[1], w_gate.shape[0], w_down.shape[0]
+    x_in = x
+    x, w_gate, w_up, w_down, fields = _check_ffn(x, w_gate, w_up, w_down, act)
+    M, D, F, O = fields[2:6]
     _like(dy, "dy", x, "x")
-    if tuple(dy.shape) != tuple(shape[:-1]) + (O,):
-        raise GddimError("dy has shape %s, expected %s" % (tuple(dy.shape), tuple(shape[:-1]) + (O,)))
+    if dy.shape != x_in.shape[:-1] + (O,):
+        raise GddimError("dy has shape %s, expected %s" % (tuple(dy.shape), tuple(x_in.shape[:-1]) + (O,)))
     if not isinstance(saved, tuple) or len(saved) != 3:
         raise GddimError("saved: expected the second result of gated_ffn(..., save=True)")
     for t, name in zip(saved, ("gate", "up", "hidden")):
         _on_gpu(t, "saved " + name)
-        if t.dtype != (x.dtype if name == "hidden" else torch.float32) or t.device != x.device:
+        if t.dtype is not (x.dtype if name == "hidden" else _torch()[0].float32) or t.get_device() != x.get_device():
             raise GddimError("saved %s is %s on %s: not what gated_ffn(..., save=True) gave for x" % (name, t.dtype, t.device))
         if tuple(t.shape) != (M, F) or not t.is_contiguous():
             raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
     dy = _rows(dy, O)
     gate, up, hidden = saved
     if (dy.data_ptr() | gate.data_ptr() | up.data_ptr() | hidden.data_ptr()) & 15 or (dy.stride(0) != O and dy.stride(0) * dy.element_size() % 16):
-        desc.unaligned = 1
+        fields = fields[:6] + (1,) + fields[7:]
     dx, dwg, dwu, dwd = x.new_empty((M, D)), x.new_empty((F, D)), x.new_empty((F, D)), x.new_empty((O, F))
-    ws = _workspace(x, desc, 1)
-    _call(x, _abi.lib().gd_gated_ffn_backward, desc, dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-          gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr(),
-          ws.data_ptr() if ws is not None else None)
-    return dx.view(shape), dwg, dwu, dwd
+    ws, ws_at = _workspace(x, fields, 1)
+    _call(x, _abi.lib().gd_gated_ffn_backward, _FFN.pack(*fields), dy.data_ptr(), dy.stride(0), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+          w_down.data_ptr(), gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr(), ws_at)
+    return dx.view(x_in.shape), dwg, dwu, dwd

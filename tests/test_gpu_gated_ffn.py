@@ -122,7 +122,7 @@ def test_nothing_is_written_beside_the_results(dev, native_lib, size, typ):
         return buf, buf[pad:pad + rows * cols].view(rows, cols)
 
     for unaligned in (0, 1):
-        d = FfnDesc(0 if typ == "f32" else 1, 0, M, D, F, O, unaligned, D, D, F)
+        d = bytes(FfnDesc(0 if typ == "f32" else 1, 0, M, D, F, O, unaligned, D, D, F))
         s = torch.cuda.current_stream().cuda_stream
         bufs = [guarded(M, F, torch.float32), guarded(M, F, torch.float32), guarded(M, F), guarded(M, O), guarded(M, D), guarded(F, D), guarded(F, D), guarded(O, F)]
         ws = [guarded(1, max(4, native_lib.gd_gated_ffn_workspace(d, b) // 4), torch.float32) for b in (0, 1)]

@@ -36,7 +36,7 @@ def _desc(**kw):
              pos_stride_axis=1, freq=64)
     d.update(kw)
     d["section"] = (ctypes.c_int * 4)(*d["section"])
-    return RotaryDesc(**d)
+    return ctypes.byref(RotaryDesc(**d))
 
 
 @pytest.mark.parametrize("bad", [
@@ -46,7 +46,7 @@ def _desc(**kw):
 def test_c_entry_points_refuse_descriptions(native_lib, bad):
     """None of these reaches a launch: the fake addresses are never read."""
     from gddim_amd._abi import Heads
-    h = Heads(64, 64, 16, 16)
+    h = ctypes.byref(Heads(64, 64, 16, 16))
     assert native_lib.gd_rotary(_desc(**bad), h, h, 1, 0, None) != 0
     assert native_lib.gd_last_error()
     assert native_lib.gd_qk_norm_rotary(_desc(**bad), h, h, h, h, 1, 1, None, None, 0, 1e-6, None) != 0
@@ -55,7 +55,7 @@ def test_c_entry_points_refuse_descriptions(native_lib, bad):
 
 def test_c_entry_points_refuse_arguments(native_lib):
     from gddim_amd._abi import Heads
-    h, null, d = Heads(64, 64, 16, 16), Heads(None, 64, 16, 16), _desc()
+    h, null, d = ctypes.byref(Heads(64, 64, 16, 16)), ctypes.byref(Heads(None, 64, 16, 16)), _desc()
     assert native_lib.gd_rotary(None, h, h, 1, 0, None) != 0
     assert native_lib.gd_rotary(d, h, null, 1, 0, None) != 0
     assert native_lib.gd_rotary(d, None, h, 1, 0, None) != 0
@@ -92,7 +92,7 @@ def _ffn(**kw):
     from gddim_amd._abi import FfnDesc
     d = dict(dtype=1, act=0, rows=4, in_=8, hidden=16, out=8, unaligned=0, ld_x=8, ld_w_in=8, ld_w_down=16)
     d.update(kw)
-    return FfnDesc(**d)
+    return ctypes.byref(FfnDesc(**d))
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=3), dict(act=3), dict(act=-1), dict(rows=-1), dict(in_=0), dict(hidden=0), dict(out=0), dict(ld_x=7), dict(ld_w_in=7),
@@ -148,3 +148,24 @@ def test_float64_block_against_autograd(kind):
     got = ref.gated_ffn(x, wg, wu, wd, kind, torch.float64, dy)
     for a, b in zip(got, (y,) + grads):
         assert (a.val - b).abs().max() < 1e-12
+
+
+def test_packed_structures_are_the_header_s(native_lib):
+    """token_ops hands the C structures over as packed bytes: the same bytes as the ctypes mirrors of the header"""
+    from gddim_amd import _abi, token_ops
+    r = _abi.RotaryDesc(1, 2, 3, 4, 2, (ctypes.c_int * 4)(8, 6, 0, 0), 1, 2, 1 << 40, 5, 6, 7, 1 << 41)
+    assert bytes(r) == token_ops._ROTARY.pack(1, 2, 3, 4, 2, 8, 6, 0, 0, 1, 2, 1 << 40, 5, 6, 7, 1 << 41)
+    assert bytes(_abi.Heads(1 << 40, 2, 3, 4)) == token_ops._HEADS.pack(1 << 40, 2, 3, 4)
+    assert bytes(_abi.FfnDesc(1, 2, 3, 4, 5, 6, 1, 8, 9, 10)) == token_ops._FFN.pack(1, 2, 3, 4, 5, 6, 1, 8, 9, 10)
+
+
+def test_rotary_axes_copies(native_lib):
+    """a copy has a table of its own; a given table is taken over by value"""
+    import copy
+    from gddim_amd import ops
+    f = torch.ones(2, dtype=torch.float64)
+    axes = ops.RotaryAxes((4,), frequencies=f, device="cpu")
+    f.zero_()
+    assert axes.frequencies.tolist() == [1.0, 1.0]
+    other = copy.deepcopy(axes)
+    assert other.frequencies.data_ptr() != axes.frequencies.data_ptr() and other.sections == axes.sections
