@@ -593,11 +593,12 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p
     }
 }
 
-// Few rows: the weights' bytes are the time, so nothing is staged.  A workgroup of 16 waves takes 16 rows of x and ROWS rows of the weights (of gate and of up),
-// a wave every 16th 128-byte line of them, straight from memory into the operand registers of 16x16 matrix-core blocks; the waves' partial sums meet in
-// LDS and are added in wave order.  All of a workgroup's bytes are on their way at once, so it takes little more than one way from memory: with 16 rows of the
-// weights a small `out` does not fill the chip, 8 or 4 (idle lanes, the matrix core has time) do.  Two launches for the block where the tiled path takes four
-// (split sums and their joins): 1 x 1024 x 2736 in bf16 10.3 us against 22.7, 33 x 1024 x 4096 22.8 against 27.2, back to back in a graph.
+// Few rows: the weights' bytes are the time, so nothing is staged.  A workgroup of 16 waves takes 16 MT rows of x and ROWS rows of the weights (of gate and of
+// up), a wave every 16th 128-byte line of them, straight from memory into the operand registers of 16x16 matrix-core blocks; the waves' partial sums meet in
+// LDS and are added in wave order.  All of a workgroup's bytes are on their way at once, so it takes little more than one way from memory -- as long as
+// there is a workgroup for every CU: MT is 3 where the weights have rows enough (gate and up of 33 x 1024 x 4096: 9.2 us with 3, 14.8 with 1), 1 where not
+// (its w_down: 9.3 with 1, 15.8 with 3), and a small w_down is cut into 8 or 4 rows (16 x 4096 -> 1024: 7.8 us with 4, 10.0 with 16; idle lanes, the matrix core has
+// time).  Two launches for the block where the tiled path takes four (split sums and their joins): 1 x 1024 x 2736 in bf16 10.2 us against 22.7.
 template <typename T> __device__ __forceinline__ f32x4 mma16(i32x4 b, i32x4 a, f32x4 c);
 template <> __device__ __forceinline__ f32x4 mma16<__bf16>(i32x4 b, i32x4 a, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
@@ -612,29 +613,32 @@ template <> __device__ __forceinline__ f32x4 mma16<float>(i32x4 b, i32x4 a, f32x
     return c;
 }
 
-template <typename T, int ROWS, int EPI>
+template <typename T, int ROWS, int MT, int EPI>
 __global__ __launch_bounds__(1024) void skinny_kernel(const GemmLaunch p) {
     constexpr int PARTS = EPI == EPI_GATED ? 2 : 1, WAVES = 16, V = 16 / sizeof(T), LINE = 128 / sizeof(T), UNROLL = 2;
-    __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][PARTS][64];
+    __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][PARTS][MT][64];
     const GemmProblem &q = p.q[0];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     // the workgroups of one slice of the weights lie on one XCD: they read it from memory once
-    const int slot = blockIdx.x >> 3, m0 = slot % q.tiles_m * 16, n0 = (slot / q.tiles_m * 8 + (blockIdx.x & 7)) * ROWS;
+    const int slot = blockIdx.x >> 3, m0 = slot % q.tiles_m * (16 * MT), n0 = (slot / q.tiles_m * 8 + (blockIdx.x & 7)) * ROWS;
     if (n0 >= q.N) return;
     // rows past the matrix read its last one: an element of the result depends on its own row and column alone, and these are not stored
-    const char *wrow[PARTS];
+    const char *wrow[PARTS], *xrow[MT];
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) wrow[s] = static_cast<const char *>(q.b[s]) + (long long)min(n0 + i, q.N - 1) * q.ldb + g * 16;
-    const char *xrow = static_cast<const char *>(q.a[0]) + (long long)min(m0 + i, q.M - 1) * q.lda + g * 16;
-    f32x4 acc[PARTS];
 #pragma unroll
-    for (int s = 0; s < PARTS; ++s) acc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < MT; ++t) xrow[t] = static_cast<const char *>(q.a[0]) + (long long)min(m0 + t * 16 + i, q.M - 1) * q.lda + g * 16;
+    f32x4 acc[PARTS][MT];
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     const int lines = (q.K + LINE - 1) / LINE;
     for (int l0 = wave; l0 < lines; l0 += WAVES * UNROLL) {
-        i32x4 fw[UNROLL][2][PARTS], fx[UNROLL][2];
+        i32x4 fw[UNROLL][2][PARTS], fx[UNROLL][2][MT];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
@@ -644,28 +648,33 @@ __global__ __launch_bounds__(1024) void skinny_kernel(const GemmLaunch p) {
                 const long long o = (long long)l * 128 + h * 64;
 #pragma unroll
                 for (int s = 0; s < PARTS; ++s) fw[u][h][s] = in && i < ROWS ? *reinterpret_cast<const i32x4 *>(wrow[s] + o) : i32x4{0, 0, 0, 0};
-                fx[u][h] = in ? *reinterpret_cast<const i32x4 *>(xrow + o) : i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < MT; ++t) fx[u][h][t] = in ? *reinterpret_cast<const i32x4 *>(xrow[t] + o) : i32x4{0, 0, 0, 0};
             }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int s = 0; s < PARTS; ++s) acc[s] = mma16<T>(fw[u][h][s], fx[u][h], acc[s]);
+                for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[s][t] = mma16<T>(fw[u][h][s], fx[u][h][t], acc[s][t]);
     }
 #pragma unroll
-    for (int s = 0; s < PARTS; ++s) part[wave][s][lane] = acc[s];
+    for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) part[wave][s][t][lane] = acc[s][t];
     __syncthreads();
-    if (wave == 0 && g * 4 < ROWS) {
+    if (wave < MT && g * 4 < ROWS) {
         f32x4 c[PARTS];
 #pragma unroll
         for (int s = 0; s < PARTS; ++s) {
-            c[s] = part[0][s][lane];
+            c[s] = part[0][s][wave][lane];
 #pragma unroll
-            for (int k = 1; k < WAVES; ++k) c[s] += part[k][s][lane];
+            for (int k = 1; k < WAVES; ++k) c[s] += part[k][s][wave][lane];
         }
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        epilogue<T, EPI>(q, p.act, m0 + i, n0 + g * 4, c[0], c[PARTS - 1], zero, zero);
+        epilogue<T, EPI>(q, p.act, m0 + wave * 16 + i, n0 + g * 4, c[0], c[PARTS - 1], zero, zero);
     }
 }
 
@@ -697,9 +706,11 @@ template <typename T, bool AKC, bool BKC, int EPI>
 int launch_gemm(const GemmLaunch &p, hipStream_t s) {
     if (p.tile == TILE_SKINNY) {
         if constexpr (AKC && BKC) {
-            if (p.skinny_rows == 16) skinny_kernel<T, 16, EPI><<<p.grid, 1024, 0, s>>>(p);
-            else if (p.skinny_rows == 8) skinny_kernel<T, 8, EPI><<<p.grid, 1024, 0, s>>>(p);
-            else skinny_kernel<T, 4, EPI><<<p.grid, 1024, 0, s>>>(p);
+            if (p.skinny_m == 3) skinny_kernel<T, 16, 3, EPI><<<p.grid, 1024, 0, s>>>(p);
+            else if (p.skinny_m == 2) skinny_kernel<T, 16, 2, EPI><<<p.grid, 1024, 0, s>>>(p);
+            else if (p.skinny_rows == 16) skinny_kernel<T, 16, 1, EPI><<<p.grid, 1024, 0, s>>>(p);
+            else if (p.skinny_rows == 8) skinny_kernel<T, 8, 1, EPI><<<p.grid, 1024, 0, s>>>(p);
+            else skinny_kernel<T, 4, 1, EPI><<<p.grid, 1024, 0, s>>>(p);
             GD_HIP(hipGetLastError());
         }
         return 0;

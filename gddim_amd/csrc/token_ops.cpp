@@ -85,17 +85,21 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
     // Few rows: the weight-streaming kernel, up to 64, and further while 16 rows of x at a time do not read more of the weights than a launch costs
-    // (skinny_kernel has the figures; 96 x 1024 x 4096 would take 41 us instead of 33, 128 x 256 x 688 takes 8.2 instead of 19.6)
-    if ((kind == GEMM_GATE_UP || kind == GEMM_DOWN) && l.direct && l.q[0].M <= 256) {
+    // (skinny_kernel has the figures; 128 x 256 x 688 takes 8.2 us instead of 19.6, 96 x 1024 x 4096 would take 41 instead of 33)
+    if ((kind == GEMM_GATE_UP || kind == GEMM_DOWN) && l.direct && l.q[0].M >= 1 && l.q[0].M <= 256) {
         GemmProblem &q = l.q[0];
         const int m_tiles = (q.M + 15) / 16;
         if (q.M <= 64 || (long long)m_tiles * (gated ? 2 : 1) * q.N * q.K * (long long)elem_size(dtype) <= (12LL << 20)) {
             l.tile = TILE_SKINNY;
             q.splits = 1;
-            q.tiles_m = m_tiles;
+            const long long slices = (q.N + 15) / 16;
+            int groups = (m_tiles + 2) / 3;
+            while (groups < m_tiles && slices * groups < cus) ++groups;
+            l.skinny_m = (m_tiles + groups - 1) / groups;
+            q.tiles_m = (m_tiles + l.skinny_m - 1) / l.skinny_m;
             l.skinny_rows = 16;
-            while (l.skinny_rows > 4 && 2LL * m_tiles * ((q.N + l.skinny_rows - 1) / l.skinny_rows) <= cus) l.skinny_rows /= 2;
-            const long long grid = (q.N + 8LL * l.skinny_rows - 1) / (8LL * l.skinny_rows) * 8 * m_tiles;
+            while (l.skinny_m == 1 && l.skinny_rows > 4 && 2LL * m_tiles * ((q.N + l.skinny_rows - 1) / l.skinny_rows) <= cus) l.skinny_rows /= 2;
+            const long long grid = (q.N + 8LL * l.skinny_rows - 1) / (8LL * l.skinny_rows) * 8 * q.tiles_m;
             if (grid > (1LL << 30)) return -1;
             l.grid = l.blocks = (int)grid;
             l.join_blocks = 0;

@@ -69,7 +69,7 @@ struct GemmLaunch {
     GemmProblem q[3];
     int problems, act, direct, join_blocks;
     int blocks, grid;            // pieces of work; workgroups
-    int skinny_rows;             // TILE_SKINNY: rows of the weights a workgroup takes
+    int skinny_m, skinny_rows;   // TILE_SKINNY: blocks of 16 rows of x and rows of the weights a workgroup takes
     GemmTile tile;
 };
 

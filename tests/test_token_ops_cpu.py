@@ -124,6 +124,17 @@ def test_c_gated_ffn_refuses_arguments(native_lib):
     assert native_lib.gd_gated_ffn_workspace(d, 1) >= 2 * 4 * 16 * 2
 
 
+def test_c_gated_ffn_workspace_over_all_sizes(native_lib):
+    """planning (on the host, for 256 compute units without a GPU) gives a size for every shape, none among them"""
+    for dtype in (0, 1, 2):
+        for rows in (0, 1, 2, 15, 16, 17, 33, 48, 64, 65, 128, 255, 256, 257, 1000, 4096, 70000, 1 << 30):
+            for in_, hidden, out in ((1, 1, 1), (8, 8, 8), (7, 13, 5), (64, 2056, 64), (1024, 4096, 1024), (264, 24, 2048)):
+                for unaligned in (0, 1):
+                    d = _ffn(dtype=dtype, rows=rows, in_=in_, hidden=hidden, out=out, unaligned=unaligned, ld_x=in_, ld_w_in=in_, ld_w_down=hidden)
+                    assert native_lib.gd_gated_ffn_workspace(d, 0) >= 0
+                    assert native_lib.gd_gated_ffn_workspace(d, 1) >= 2 * rows * hidden * (4 if dtype == 0 else 2)
+
+
 def test_gated_ffn_needs_a_gpu(native_lib):
     from gddim_amd import ops
     from gddim_amd._abi import GddimError
