@@ -113,8 +113,9 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     // stage's time per stage, and a fixed time for the way in and out.  Split sums are written and read again by the join.  The constants are fits to y
     // = h Wd^T of 16384 x 1024, K = 256 .. 4096, in bf16 (256: 16.5, 23.6, 36.8, 127.9 us; 128: 18.4, 25.6, 40.5, 148.9) and to one and two 128 tiles a CU
     // (21.6, 24.9 us at K = 1024; in float32 2.3 and 1.8 us a stage and tile); operands whose k is not adjacent cost the small tile more (the weights'
-    // gradients of 16384 x 1024 x 4096: 432 us with 256, 554 with 128).
-    const double stage256 = kind == GEMM_DW ? 1.7 : 1.9, stage128 = kind == GEMM_DW ? 0.72 : kind == GEMM_DHIDDEN || kind == GEMM_DX ? 0.65 : 0.57;
+    // gradients of 16384 x 1024 x 4096: 432 us with 256, 554 with 128), and where every CU multiplies, the clock falls: split four ways over all of them these
+    // gradients' 192 tiles take 421 us and the join 45.
+    const double stage128 = kind == GEMM_DW ? 0.72 : kind == GEMM_DHIDDEN || kind == GEMM_DX ? 0.65 : 0.57;
     const long long stages = stages_of(l.q[0]);
     double best = 1e30;
     long long best_split = 1;
@@ -130,7 +131,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
         for (long long s = 1; s <= 16 && s <= stages && (s == 1 || stages / s >= 4); ++s) {
             const double per = (double)((stages + s - 1) / s), c = (double)((n * s + cus - 1) / cus);
             double us;
-            if (t == 256) us = c * (stage256 * per + 3) + 5;
+            if (t == 256) us = c * ((kind != GEMM_DW ? 1.9 : n * s < cus ? 1.7 : 2.1) * per + 3) + 5;
             else if (dtype == GD_F32) us = c <= 1 ? 2.3 * per + 5 : 1.8 * c * per + 8;
             else us = c <= 1 ? 1.05 * per + 5 : stage128 * c * per + 8;
             if (s > 1) us += 4 + (double)s * out * 8 / 4.5e6;
