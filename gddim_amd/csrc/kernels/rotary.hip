@@ -15,13 +15,13 @@
 //
 // Layout: a lane holds W pairs = two vectors of W channels.  (i, i + R/2) pairs: vector 0 from the first half, vector 1 from the second;
 // (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head: the weight-gradient sums stay in
-// registers (norm weights come from LDS, queries and keys apart).  LP lanes (a power of two) hold a head: the norm's sums are log2 LP permutes, 64 / LP
+// registers (norm weights come from LDS, queries and keys apart).  lp lanes hold a head (with the norm a power of two: its sums are log2 lp permutes), 64 / lp
 // heads are in flight per wave.  Channels that pass through are pairs with phi = 0.
 //
 // W is 16 bytes of a type where pairs, strides and addresses allow it (the gradient in 16-bit types: 8), 8 bytes else, one pair where nothing is aligned.
 //
-// Measured, against the bytes at the 5.1 TB/s of a large copy: rotation of 46800 x 16 x 128 bf16 (383 MB) 78 us, 4.9 TB/s; norm and rotation of 65536 tokens x
-// (4 + 4) x 64 float32 (268 MB) 52 us, 5.1 TB/s; of 16382 x (16 + 4) x 128 bf16 45 us, 3.7 TB/s, and its gradient (252 MB) 69 us, 3.7 TB/s, + 5 us for
+// Measured, against the bytes at the 5.1 TB/s of a large copy: rotation of 46800 x 16 x 128 bf16 (383 MB) 80 us, 4.8 TB/s; norm and rotation of 65536 tokens x
+// (4 + 4) x 64 float32 (268 MB) 56 us, 4.8 TB/s; of 16382 x (16 + 4) x 128 bf16 (168 MB) 42 us, 4.0 TB/s, and its gradient (252 MB) 74 us, 3.4 TB/s, + 5 us for
 // the weights' sums.
 #include "../common.h"
 #include "../token_ops.h"
@@ -95,20 +95,19 @@ __device__ __forceinline__ float inverse_root(float v) {
 
 // NC: chunks of W pairs per lane (1 unless one head needs more than 64 lanes)
 template <typename T, int W, int NC, bool HALVES, int MODE>
-__global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void rotary_kernel(const RotaryParams p, const int lp_log2) {
+__global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void rotary_kernel(const RotaryParams p, const int lp_log2, const int lp) {
     constexpr bool NORM = MODE != ROT_PLAIN, BWD = MODE == ROT_NORM_BWD;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
-    const int LP = 1 << lp_log2;
     const int pairs = (p.D + 1) / 2, R2 = p.R / 2;
     const int chunks = (pairs + W - 1) / W;  // W > 1: whole (the launcher's rule)
-    float2 *table = reinterpret_cast<float2 *>(smem) + wave * (chunks * W);
+    float2 *table = reinterpret_cast<float2 *>(smem) + wave * (p.group * chunks * W);
     const int wpad = (p.D + 3) & ~3;
-    float *weights = reinterpret_cast<float *>(smem + (size_t)waves * chunks * W * sizeof(float2));  // [2][wpad], float32
-    const int sub = lane >> lp_log2;
-    const int row_step = 64 >> lp_log2;
+    float *weights = reinterpret_cast<float *>(smem + (size_t)waves * p.group * chunks * W * sizeof(float2));  // [2][wpad], float32
+    const int row_step = 64 / lp;
+    const int sub = lane / lp, in_head = lane - sub * lp;  // (sub == row_step: lanes left over where lp is no power of two)
 
     if constexpr (NORM) {
         for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
@@ -123,12 +122,12 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
     bool on0[NC], on1[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        ch[c] = (lane & (LP - 1)) + 64 * c;
+        ch[c] = in_head + 64 * c;
         const int pr = ch[c] * W;
         if (!HALVES) { e0[c] = 2 * pr; e1[c] = 2 * pr + W; }
         else if (pr < R2) { e0[c] = pr; e1[c] = R2 + pr; }
         else { e0[c] = p.R + (pr - R2); e1[c] = p.R + (p.D - p.R + 1) / 2 + (pr - R2); }
-        on0[c] = ch[c] < chunks;
+        on0[c] = ch[c] < chunks && sub < row_step;
         on1[c] = on0[c] && e1[c] < p.D;  // an odd head has one channel without a partner (W == 1)
     }
     float dw[2][NC][2 * W];
@@ -142,18 +141,25 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
     const float inv_d = 1.f / (float)p.D;
     const int rows = p.heads[0] + p.heads[1];
 
-    // an item: a token (b, n) and the heads [r0, r_end) of it
+    // An item: `group` tokens from (b, n) on, or a share of one token's heads; rows [i0, i1) of it, row i being head i % heads of token i / heads
     struct Item {
-        int b, n, r0, r_end;
+        int b, n, i0, i1;
     };
+    const unsigned tokens = (unsigned)p.batch * (unsigned)p.tokens;
     auto locate = [&](unsigned id) __attribute__((always_inline)) {
         Item t;
-        const int token = (int)(id / (unsigned)p.items_per_token);
-        t.b = token / p.tokens;
-        t.n = token - t.b * p.tokens;
-        t.r0 = ((int)id - token * p.items_per_token) * p.rows_per_item;
-        t.r_end = min(rows, t.r0 + p.rows_per_item);
+        const unsigned q = id / (unsigned)p.items_per_token, token = q * p.group;
+        t.b = (int)(token / (unsigned)p.tokens);
+        t.n = (int)(token - (unsigned)t.b * p.tokens);
+        t.i0 = (int)(id - q * p.items_per_token) * p.rows_per_item;
+        t.i1 = p.group > 1 ? (int)min((unsigned)p.group, tokens - token) * rows : min(rows, t.i0 + p.rows_per_item);
         return t;
+    };
+    // token k of an item
+    auto step_token = [&](const Item &t, int k, int &b, int &n) __attribute__((always_inline)) {
+        b = t.b;
+        n = t.n + k;
+        while (n >= p.tokens) { n -= p.tokens; ++b; }
     };
     auto axis_of = [&](int pr) __attribute__((always_inline)) {
         int a = 0;
@@ -161,20 +167,27 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
         for (int i = 0; i < ROT_MAX_AXES - 1; ++i) a += (i + 1 < p.n_axes && pr >= p.axis_end[i]);
         return a;
     };
-    // the lane's first pair keeps its frequency, and its position is read an item ahead
-    const int axis0 = axis_of(lane);
-    const double freq0 = lane < R2 ? p.freq[lane] : 0.0;
-    auto pos_of = [&](const Item &t) __attribute__((always_inline)) { return lane < R2 ? load_pos(p, t.b, t.n, axis0) : 0.0; };
+    // The table holds P pairs of every token of the item.  A lane's first one keeps its frequency, and its position is read an item ahead
+    const int P = chunks * W, entries = p.group * P;
+    const int k0 = lane / P, pr0 = lane - k0 * P;
+    const bool turns0 = lane < entries && pr0 < R2;
+    const int axis0 = axis_of(pr0);
+    const double freq0 = turns0 ? p.freq[pr0] : 0.0;
+    auto pos_of = [&](const Item &t, int k, int axis) __attribute__((always_inline)) {
+        int b, n;
+        step_token(t, k, b, n);
+        return b < p.batch ? load_pos(p, b, n, axis) : 0.0;  // (the last item may hold fewer tokens)
+    };
 
     vec<T, W> v0[NC], v1[NC], g0[NC], g1[NC];
-    auto at = [&](const HeadsView *hv, const Item &t, int r) __attribute__((always_inline)) {
+    auto at = [&](const HeadsView *hv, int b, int n, int r) __attribute__((always_inline)) {
         const int seg = r >= p.heads[0];
         const HeadsView &h = hv[seg];
-        return static_cast<T *>(h.p) + (t.b * h.sb + t.n * h.sn + (r - (seg ? p.heads[0] : 0)) * h.sh);
+        return static_cast<T *>(h.p) + (b * h.sb + n * h.sn + (r - (seg ? p.heads[0] : 0)) * h.sh);
     };
-    auto load = [&](const Item &t, int r) __attribute__((always_inline)) {
-        const T *src = at(p.x, t, r);
-        const T *gsrc = BWD ? at(p.dy, t, r) : nullptr;
+    auto load = [&](int b, int n, int r) __attribute__((always_inline)) {
+        const T *src = at(p.x, b, n, r);
+        const T *gsrc = BWD ? at(p.dy, b, n, r) : nullptr;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             v0[c] = vec<T, W>{}; v1[c] = vec<T, W>{};
@@ -187,124 +200,147 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
             }
         }
     };
-
-    unsigned id = blockIdx.x * waves + wave;
-    Item cur{0, 0, 0, 0};
-    double pos0 = 0.0;
-    if (id < p.items) {
-        cur = locate(id);
-        pos0 = pos_of(cur);
-        if (cur.r0 + sub < cur.r_end) load(cur, cur.r0 + sub);
-    }
-    while (id < p.items) {
-        for (int pr = lane; pr < chunks * W; pr += 64) {
-            float2 cs = make_float2(1.f, 0.f);
-            if (pr < R2) {
-                cs = pr == lane ? cos_sin(pos0, freq0) : cos_sin(load_pos(p, cur.b, cur.n, axis_of(pr)), p.freq[pr]);
-                cs.y *= p.sign;
-            }
-            table[pr] = cs;
-        }
-        // the next item's position and, behind this one's last heads, its first are on their way while this one is worked on
-        const unsigned next_id = id + gridDim.x * waves;
-        Item next{0, 0, 0, 0};
-        if (next_id < p.items) {
-            next = locate(next_id);
-            pos0 = pos_of(next);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        float cs[NC][W], sn[NC][W];
+    float cs[NC][W], sn[NC][W];
+    auto read_table = [&](const float2 *from) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const float2 t = table[on0[c] ? ch[c] * W + i : 0];
+                const float2 t = from[on0[c] ? ch[c] * W + i : 0];
                 cs[c][i] = t.x; sn[c][i] = t.y;
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();  // the table is read before the next item overwrites it
-
-        // all lanes of the wave walk the same number of steps: the sums below need every lane of a head
-        for (int r00 = cur.r0; r00 < cur.r_end; r00 += row_step) {
-            const int r = r00 + sub;
-            const bool row_on = r < cur.r_end;
-            const int seg = r >= p.heads[0];
-            float a[NC][2 * W], g[NC][2 * W];
+    };
+    float a[NC][2 * W], g[NC][2 * W];
+    auto convert = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            to_f32<T, W>(v0[c], a[c]); to_f32<T, W>(v1[c], a[c] + W);
+            if constexpr (BWD) { to_f32<T, W>(g0[c], g[c]); to_f32<T, W>(g1[c], g[c] + W); }
+        }
+    };
+    // head r of token (b, n), in a and g; every lane of the wave takes part in the sums
+    auto work = [&](int b, int n, int r, bool row_on) __attribute__((always_inline)) {
+        const int seg = r >= p.heads[0];
+        // index of a pair's two channels among the lane's 2W
+        auto turn = [&](float *y, int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int ia = HALVES ? i : 2 * i, ib = HALVES ? W + i : 2 * i + 1;
+                const float u = y[ia], v = y[ib];
+                y[ia] = u * cs[c][i] - v * sn[c][i];
+                y[ib] = u * sn[c][i] + v * cs[c][i];
+            }
+        };
+        if constexpr (NORM) {
+            float ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2 * W; ++i) ss += a[c][i] * a[c][i];
+            float w[NC][2 * W];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                to_f32<T, W>(v0[c], a[c]); to_f32<T, W>(v1[c], a[c] + W);
-                if constexpr (BWD) { to_f32<T, W>(g0[c], g[c]); to_f32<T, W>(g1[c], g[c] + W); }
-            }
-            if (r00 + row_step < cur.r_end) {
-                if (r + row_step < cur.r_end) load(cur, r + row_step);
-            } else if (next.r0 + sub < next.r_end) load(next, next.r0 + sub);
-
-            // index of a pair's two channels among the lane's 2W
-            auto turn = [&](float *y, int c) __attribute__((always_inline)) {
+                const float *ws = weights + (seg ? wpad : 0);
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
-                    const int ia = HALVES ? i : 2 * i, ib = HALVES ? W + i : 2 * i + 1;
-                    const float u = y[ia], v = y[ib];
-                    y[ia] = u * cs[c][i] - v * sn[c][i];
-                    y[ib] = u * sn[c][i] + v * cs[c][i];
+                    w[c][i] = ws[on0[c] ? e0[c] + i : 0];
+                    w[c][W + i] = ws[on1[c] ? e1[c] + i : 0];
                 }
-            };
-            if constexpr (NORM) {
-                float ss = 0.f;
+            }
+            if constexpr (BWD) {
+                float gx = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    turn(g[c], c);
+#pragma unroll
+                    for (int i = 0; i < 2 * W; ++i) gx += g[c][i] * w[c][i] * a[c][i];
+                }
+                ss = head_sum(ss, lp_log2);
+                gx = head_sum(gx, lp_log2);
+                const float rho = inverse_root(ss * inv_d + p.eps);
+                const float k = gx * inv_d * rho * rho;  // mean(g w xh) rho: xh mean(g w xh) = x k
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int i = 0; i < 2 * W; ++i) ss += a[c][i] * a[c][i];
-                float w[NC][2 * W];
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const float *ws = weights + (seg ? wpad : 0);
-#pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        w[c][i] = ws[on0[c] ? e0[c] + i : 0];
-                        w[c][W + i] = ws[on1[c] ? e1[c] + i : 0];
+                    for (int i = 0; i < 2 * W; ++i) {
+                        const float gi = row_on ? g[c][i] * (a[c][i] * rho) : 0.f;
+                        dw[0][c][i] += seg ? 0.f : gi;
+                        dw[1][c][i] += seg ? gi : 0.f;
+                        a[c][i] = rho * (g[c][i] * w[c][i] - a[c][i] * k);
                     }
-                }
-                if constexpr (BWD) {
-                    float gx = 0.f;
+            } else {
+                const float rho = inverse_root(head_sum(ss, lp_log2) * inv_d + p.eps);
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        turn(g[c], c);
+                for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int i = 0; i < 2 * W; ++i) gx += g[c][i] * w[c][i] * a[c][i];
-                    }
-                    ss = head_sum(ss, lp_log2);
-                    gx = head_sum(gx, lp_log2);
-                    const float rho = inverse_root(ss * inv_d + p.eps);
-                    const float k = gx * inv_d * rho * rho;  // mean(g w xh) rho: xh mean(g w xh) = x k
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int i = 0; i < 2 * W; ++i) {
-                            const float gi = row_on ? g[c][i] * (a[c][i] * rho) : 0.f;
-                            dw[0][c][i] += seg ? 0.f : gi;
-                            dw[1][c][i] += seg ? gi : 0.f;
-                            a[c][i] = rho * (g[c][i] * w[c][i] - a[c][i] * k);
-                        }
-                } else {
-                    const float rho = inverse_root(head_sum(ss, lp_log2) * inv_d + p.eps);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int i = 0; i < 2 * W; ++i) a[c][i] = a[c][i] * rho * w[c][i];
-                }
-            }
-            if (row_on) {
-                T *dst = at(p.out, cur, r);
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    if constexpr (!BWD) turn(a[c], c);
-                    if (on0[c]) *reinterpret_cast<vec<T, W> *>(dst + e0[c]) = from_f32<T, W>(a[c]);
-                    if (on1[c]) *reinterpret_cast<vec<T, W> *>(dst + e1[c]) = from_f32<T, W>(a[c] + W);
-                }
+                    for (int i = 0; i < 2 * W; ++i) a[c][i] = a[c][i] * rho * w[c][i];
             }
         }
+        if (row_on) {
+            T *dst = at(p.out, b, n, r);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (!BWD) turn(a[c], c);
+                if (on0[c]) *reinterpret_cast<vec<T, W> *>(dst + e0[c]) = from_f32<T, W>(a[c]);
+                if (on1[c]) *reinterpret_cast<vec<T, W> *>(dst + e1[c]) = from_f32<T, W>(a[c] + W);
+            }
+        }
+    };
+
+    // the rows that are on their way: token k of their item, (b, n), head r
+    int lk = 0, lb = 0, ln = 0, lr = 0;
+    bool lon = false;
+    auto fetch = [&](const Item &t, int base) __attribute__((always_inline)) {
+        const int i = base + sub;
+        lon = i < t.i1 && sub < row_step;
+        lk = p.group > 1 ? i / rows : 0;
+        lr = i - lk * rows;
+        step_token(t, lon ? lk : 0, lb, ln);
+        if (lon) load(lb, ln, lr);
+    };
+
+    unsigned id = blockIdx.x * waves + wave;
+    const unsigned stride = gridDim.x * waves;
+    Item cur{0, 0, 0, 0};
+    double pos0 = 0.0;
+    if (id < p.items) {
+        cur = locate(id);
+        if (turns0) pos0 = pos_of(cur, k0, axis0);
+        fetch(cur, cur.i0);
+    }
+    while (id < p.items) {
+        if (lane < entries) {
+            float2 c = turns0 ? cos_sin(pos0, freq0) : make_float2(1.f, 0.f);
+            c.y *= p.sign;
+            table[lane] = c;
+        }
+        for (int e = lane + 64; e < entries; e += 64) {
+            const int k = e / P, pr = e - k * P;
+            float2 c = make_float2(1.f, 0.f);
+            if (pr < R2) c = cos_sin(pos_of(cur, k, axis_of(pr)), p.freq[pr]);
+            c.y *= p.sign;
+            table[e] = c;
+        }
+        // the next item's positions and, behind this one's last rows, its first are on their way while this one is worked on
+        const unsigned next_id = id + stride;
+        Item next{0, 0, 0, 0};
+        if (next_id < p.items) {
+            next = locate(next_id);
+            if (turns0) pos0 = pos_of(next, k0, axis0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int base = cur.i0; base < cur.i1; base += row_step) {
+            const int b = lb, n = ln, r = lr;
+            const bool on = lon;
+            if (p.group > 1 || base == cur.i0) read_table(table + (on ? lk : 0) * P);
+            convert();
+            if (base + row_step < cur.i1) fetch(cur, base + row_step);
+            else if (next_id < p.items) fetch(next, next.i0);
+            work(b, n, r, on);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();  // the table is read before the next item overwrites it
         id = next_id;
         cur = next;
     }
@@ -321,7 +357,7 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
 #pragma unroll
                 for (int i = 0; i < 2 * W; ++i) {
                     float t = dw[s][c][i];
-                    for (int m = LP; m < 64; m <<= 1) t += __shfl_xor(t, m);
+                    for (int m = lp; m < 64; m <<= 1) t += __shfl_xor(t, m);
                     const int e = i < W ? e0[c] + i : e1[c] + i - W;
                     if (sub == 0 && (i < W ? on0[c] : on1[c])) red[(wave * 2 + s) * p.D + e] = t;
                 }
@@ -362,16 +398,16 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float *part, int 
 }
 
 template <typename T, int W, int NC, bool HALVES>
-int launch_mode(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks, void *dw0, void *dw1, hipStream_t s) {
+int launch_mode(const RotaryParams &p, RotaryMode mode, int lp_log2, int lp, int blocks, void *dw0, void *dw1, hipStream_t s) {
     const int chunks = ((p.D + 1) / 2 + W - 1) / W;
     const int waves = mode == ROT_NORM_BWD ? ROT_BWD_THREADS / 64 : 4;
-    size_t lds = (size_t)waves * chunks * W * sizeof(float2) + (mode == ROT_PLAIN ? 0 : 2 * ((p.D + 3) & ~3) * sizeof(float));
+    size_t lds = (size_t)waves * p.group * chunks * W * sizeof(float2) + (mode == ROT_PLAIN ? 0 : 2 * ((p.D + 3) & ~3) * sizeof(float));
     switch (mode) {
-        case ROT_PLAIN: rotary_kernel<T, W, NC, HALVES, ROT_PLAIN><<<blocks, 256, lds, s>>>(p, lp_log2); break;
-        case ROT_NORM: rotary_kernel<T, W, NC, HALVES, ROT_NORM><<<blocks, 256, lds, s>>>(p, lp_log2); break;
+        case ROT_PLAIN: rotary_kernel<T, W, NC, HALVES, ROT_PLAIN><<<blocks, 256, lds, s>>>(p, lp_log2, lp); break;
+        case ROT_NORM: rotary_kernel<T, W, NC, HALVES, ROT_NORM><<<blocks, 256, lds, s>>>(p, lp_log2, lp); break;
         case ROT_NORM_BWD:
             if (lds < (size_t)waves * 2 * p.D * sizeof(float)) lds = (size_t)waves * 2 * p.D * sizeof(float);
-            if constexpr (W * sizeof(T) <= 8 || sizeof(T) == 4) rotary_kernel<T, W, NC, HALVES, ROT_NORM_BWD><<<blocks, ROT_BWD_THREADS, lds, s>>>(p, lp_log2);
+            if constexpr (W * sizeof(T) <= 8 || sizeof(T) == 4) rotary_kernel<T, W, NC, HALVES, ROT_NORM_BWD><<<blocks, ROT_BWD_THREADS, lds, s>>>(p, lp_log2, lp);
             GD_HIP(hipGetLastError());
             rotary_dw_kernel<T><<<(2 * p.D + 15) / 16, 1024, 0, s>>>(p.dw_part, blocks, p.D, dw0, dw1, p.w_f32);
             break;
@@ -381,15 +417,15 @@ int launch_mode(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks,
 }
 
 template <typename T, int W, int NC>
-int launch_pairs(const RotaryParams &p, RotaryMode mode, int lp_log2, int blocks, void *dw0, void *dw1, hipStream_t s) {
-    return p.halves ? launch_mode<T, W, NC, true>(p, mode, lp_log2, blocks, dw0, dw1, s)
-                    : launch_mode<T, W, NC, false>(p, mode, lp_log2, blocks, dw0, dw1, s);
+int launch_pairs(const RotaryParams &p, RotaryMode mode, int lp_log2, int lp, int blocks, void *dw0, void *dw1, hipStream_t s) {
+    return p.halves ? launch_mode<T, W, NC, true>(p, mode, lp_log2, lp, blocks, dw0, dw1, s)
+                    : launch_mode<T, W, NC, false>(p, mode, lp_log2, lp, blocks, dw0, dw1, s);
 }
 
-// vectors of W channels: every address a multiple of their size, pairs and pass-through channels whole vectors
+// vectors of W channels: every address a multiple of their size, the halves' pairs and pass-through channels whole vectors
 bool vec_ok(const RotaryParams &p, int W, int elem, bool bwd) {
     const size_t bytes = (size_t)W * elem;
-    if (p.D % (2 * W) || p.R % (2 * W)) return false;
+    if (p.D % (2 * W) || (p.halves && p.R % (2 * W))) return false;  // (2i, 2i + 1) pairs may end inside a lane's: the rest pass through
     auto ok = [&](const HeadsView &h) {
         return (size_t)h.p % bytes == 0 && h.sb % W == 0 && h.sn % W == 0 && h.sh % W == 0;
     };
@@ -407,7 +443,8 @@ int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStrea
     const int chunks = ((p.D + 1) / 2 + W - 1) / W;
     int lp_log2 = 0;
     while (lp_log2 < 6 && (1 << lp_log2) < chunks) ++lp_log2;
-    const int rows = p.heads[0] + p.heads[1], row_step = 64 >> lp_log2;
+    const int lp = mode == ROT_PLAIN && chunks < 64 ? chunks : 1 << lp_log2;  // lanes of a head: without sums over them, no more than it has chunks
+    const int rows = p.heads[0] + p.heads[1], row_step = 64 / lp;
     const long long tokens = (long long)p.batch * p.tokens;
     if (tokens == 0) {
         if (bwd) rotary_dw_kernel<T><<<(2 * p.D + 15) / 16, 1024, 0, s>>>(p.dw_part, 0, p.D, dw0, dw1, p.w_f32);
@@ -423,13 +460,29 @@ int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStrea
     p.rows_per_item = (int)((steps + shares - 1) / shares) * row_step;
     p.items_per_token = (rows + p.rows_per_item - 1) / p.rows_per_item;
     p.items = (unsigned)(tokens * p.items_per_token);  // < 2^31: shares are taken only where tokens are few
+    // A step or a few a token are mostly the way from its position to its angles: an item of several tokens then, until it is four steps of the wave (and
+    // its table 256 pairs), as long as there are items enough (6 x 13278 tokens of one 64-channel head in fp16: 16.5 us a
+    // call instead of 36; 13 x 10525 of three of 16 in float32 15 instead of 53)
+    const int P = chunks * W;
+    p.group = 1;
+    if (shares == 1 && rows <= 4 * row_step) {
+        long long group = (4LL * row_step + rows - 1) / rows;
+        if (group > 256 / P) group = 256 / P;
+        if (group > tokens / want) group = tokens / want;
+        if (group > 1) {
+            p.group = (int)group;
+            p.items = (unsigned)((tokens + group - 1) / group);
+            p.items_per_token = 1;
+        }
+    }
     const unsigned per_block = bwd ? ROT_BWD_THREADS / 64 : 4;
     unsigned blocks = (p.items + per_block - 1) / per_block;
     if (blocks > (unsigned)max_blocks) blocks = max_blocks;
-    if (W == WV && chunks <= 64) return launch_pairs<T, WV, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
-    if (W == WV / 2 && W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
-    if (chunks <= 64) return launch_pairs<T, 1, 1>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
-    return launch_pairs<T, 1, 4>(p, mode, lp_log2, (int)blocks, dw0, dw1, s);
+    if (W == WV && chunks <= 64) return launch_pairs<T, WV, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    if (W == WV / 2 && W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    if (chunks <= 64) return launch_pairs<T, 1, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    if (chunks <= 128) return launch_pairs<T, 1, 2>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    return launch_pairs<T, 1, 4>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
 }
 
 }  // namespace

@@ -38,6 +38,7 @@ struct RotaryParams {
     float *dw_part;  // [blocks][2][D]
     // filled in by the launcher
     int rows_per_item, items_per_token;
+    int group;  // tokens of an item
     unsigned items;
 };
 

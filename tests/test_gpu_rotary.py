@@ -61,6 +61,9 @@ SHAPES = [
     (1, 9, 33, 3, 96, (32, 32, 32), "packed"),
     (1, 4, 2, 2, 64, (32, 32), "channels"),
     (2, 4301, 2, 1, 16, (4, 6, 6), "dense"),   # tokens enough to fill the chip: whole tokens per wave
+    (3, 8191, 1, 1, 64, (24, 16, 24), "bhnd"),  # ... and several small ones
+    (2, 20011, 3, 1, 16, (16,), "dense"),
+    (1, 33001, 2, 2, 7, (4, 2), "packed"),
 ]
 
 
