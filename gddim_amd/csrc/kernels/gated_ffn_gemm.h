@@ -71,18 +71,28 @@ template <int ACT> __device__ __forceinline__ void act_grad(float z, float &a, f
 }
 
 // ---- epilogues on four adjacent columns of one row ----
-template <typename T> __device__ __forceinline__ void store4(void *p, long long o, f32x4 v, int n_left, bool whole) {
+// four elements at any address (rows of odd length begin anywhere; global memory takes whole accesses there, too)
+template <typename T> __device__ __forceinline__ void store_quad(T *d, f32x4 v) {
+    const typename quad<T>::type t = __builtin_convertvector(v, typename quad<T>::type);
+    __builtin_memcpy(d, &t, sizeof t);
+}
+template <typename T> __device__ __forceinline__ f32x4 load_quad(const T *d) {
+    typename quad<T>::type t;
+    __builtin_memcpy(&t, d, sizeof t);
+    return __builtin_convertvector(t, f32x4);
+}
+template <typename T> __device__ __forceinline__ void store4(void *p, long long o, f32x4 v, int n_left) {
     T *d = static_cast<T *>(p) + o;
-    if (whole) *reinterpret_cast<typename quad<T>::type *>(d) = __builtin_convertvector(v, typename quad<T>::type);
+    if (n_left >= 4) store_quad<T>(d, v);
     else
-        for (int i = 0; i < 4 && i < n_left; ++i) d[i] = (T)v[i];
+        for (int i = 0; i < n_left; ++i) d[i] = (T)v[i];
 }
 
-template <typename T> __device__ __forceinline__ f32x4 load4(const void *p, long long o, int n_left, bool whole) {
+template <typename T> __device__ __forceinline__ f32x4 load4(const void *p, long long o, int n_left) {
     const T *d = static_cast<const T *>(p) + o;
-    if (whole) return __builtin_convertvector(*reinterpret_cast<const typename quad<T>::type *>(d), f32x4);
+    if (n_left >= 4) return load_quad<T>(d);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < 4 && i < n_left; ++i) v[i] = (float)d[i];
+    for (int i = 0; i < n_left; ++i) v[i] = (float)d[i];
     return v;
 }
 
@@ -91,17 +101,16 @@ template <typename T, int EPI, int ACT>
 __device__ __forceinline__ void epilogue_act(const GemmProblem &q, int m, int n, f32x4 c0, f32x4 c1, f32x4 g, f32x4 u) {
     const int left = q.N - n;
     if (m >= q.M || left <= 0) return;
-    const bool whole = q.quads && left >= 4;
     const long long o = (long long)m * q.N + n;
-    if constexpr (EPI == EPI_STORE) store4<T>(q.out[0], o, c0, left, whole);
+    if constexpr (EPI == EPI_STORE) store4<T>(q.out[0], o, c0, left);
     else if constexpr (EPI == EPI_GATED) {
         f32x4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = act_value<ACT>(c0[e]) * c1[e];
-        store4<T>(q.out[0], o, h, left, whole);
+        store4<T>(q.out[0], o, h, left);
         if (q.out[1]) {
-            store4<float>(q.out[1], o, c0, left, whole);
-            store4<float>(q.out[2], o, c1, left, whole);
+            store4<float>(q.out[1], o, c0, left);
+            store4<float>(q.out[2], o, c1, left);
         }
     } else {
         f32x4 dg, du;
@@ -112,8 +121,8 @@ __device__ __forceinline__ void epilogue_act(const GemmProblem &q, int m, int n,
             dg[e] = c0[e] * u[e] * da;
             du[e] = c0[e] * a;
         }
-        store4<T>(q.out[0], o, dg, left, whole);
-        store4<T>(q.out[1], o, du, left, whole);
+        store4<T>(q.out[0], o, dg, left);
+        store4<T>(q.out[1], o, du, left);
     }
 }
 
@@ -129,10 +138,9 @@ __device__ __forceinline__ void load_kept(const GemmProblem &q, int m, int n, f3
     const int left = q.N - n;
     g = u = f32x4{0.f, 0.f, 0.f, 0.f};
     if (m >= q.M || left <= 0) return;
-    const bool whole = q.quads && left >= 4;
     const long long o = (long long)m * q.N + n;
-    g = load4<float>(q.in[0], o, left, whole);
-    u = load4<float>(q.in[1], o, left, whole);
+    g = load4<float>(q.in[0], o, left);
+    u = load4<float>(q.in[1], o, left);
 }
 
 // of a 32 x 32 block in the accumulators, lane l holds row l % 32 and columns 8 e + 4 (l / 32) .. + 3, e = 0 .. 3
@@ -298,13 +306,12 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// 32 rows of accumulators from LDS through the epilogue.  Inside the matrix with whole quads (all of a large one) the loop is stripped of bounds, of 64-bit
+// 32 rows of accumulators from LDS through the epilogue.  Inside the matrix (all of a large one) the loop is stripped of bounds, of 64-bit
 // address arithmetic and of the choice of activation: with those, instructions bound it (13 us of a tile's 43 at 16384 x 1024 x 4096).
 template <typename T, int EPI, int ACT>
 __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mine, int m, int n, int lane) {
     constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
     constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR, ITER = 32 / RPI;
-    typedef typename quad<T>::type Q;
     const int row = lane / LPR, piece = lane % LPR;
     const long long first = (long long)m * q.N + n;
     const unsigned at = (unsigned)row * (unsigned)q.N + piece * 4, next = (unsigned)q.N * RPI;  // elements; 32 rows < 2^31 bytes (the launcher's rule)
@@ -316,8 +323,8 @@ __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mi
     if constexpr (BWD) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
-            g[k] = *reinterpret_cast<const f32x4 *>(gi + at + k * next);
-            u[k] = *reinterpret_cast<const f32x4 *>(ui + at + k * next);
+            g[k] = load_quad<float>(gi + at + k * next);
+            u[k] = load_quad<float>(ui + at + k * next);
         }
     }
 #pragma unroll
@@ -325,16 +332,16 @@ __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mi
         const int r = k * RPI + row;
         const unsigned o = at + k * next;
         const f32x4 c0 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + ((piece ^ (r & 15)) << 4));
-        if constexpr (EPI == EPI_STORE) *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(c0, Q);
+        if constexpr (EPI == EPI_STORE) store_quad<T>(o0 + o, c0);
         else if constexpr (GATED) {
             const f32x4 c1 = *reinterpret_cast<const f32x4 *>(mine + r * 256 + (((piece + 8) ^ (r & 15)) << 4));
             f32x4 h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = act_value<ACT>(c0[e]) * c1[e];
-            *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(h, Q);
+            store_quad<T>(o0 + o, h);
             if (g0) {
-                *reinterpret_cast<f32x4 *>(g0 + o) = c0;
-                *reinterpret_cast<f32x4 *>(u0 + o) = c1;
+                store_quad<float>(g0 + o, c0);
+                store_quad<float>(u0 + o, c1);
             }
         } else {
             f32x4 dg, du;
@@ -345,8 +352,8 @@ __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mi
                 dg[e] = c0[e] * u[k][e] * da;
                 du[e] = c0[e] * a;
             }
-            *reinterpret_cast<Q *>(o0 + o) = __builtin_convertvector(dg, Q);
-            *reinterpret_cast<Q *>(o1 + o) = __builtin_convertvector(du, Q);
+            store_quad<T>(o0 + o, dg);
+            store_quad<T>(o1 + o, du);
         }
     }
 }
@@ -355,7 +362,7 @@ template <typename T, int EPI>
 __device__ __forceinline__ void rows_out(const GemmProblem &q, int act, const char *mine, int m, int n, int lane) {
     constexpr bool GATED = EPI == EPI_GATED;
     constexpr int LPR = GATED ? 8 : 16, RPI = 64 / LPR;
-    if (q.quads && m + 32 <= q.M && n + LPR * 4 <= q.N) {
+    if (q.short_rows && m + 32 <= q.M && n + LPR * 4 <= q.N) {
         if (EPI == EPI_STORE || act == GD_ACT_SILU) rows_inside<T, EPI, GD_ACT_SILU>(q, mine, m, n, lane);
         else if (act == GD_ACT_GELU) rows_inside<T, EPI, GD_ACT_GELU>(q, mine, m, n, lane);
         else rows_inside<T, EPI, GD_ACT_GELU_TANH>(q, mine, m, n, lane);

@@ -173,9 +173,7 @@ int run_gemm(GemmLaunch &l, int dtype, GemmKind kind, float *partial, hipStream_
     GD_CHECK(plan_gemm(l, dtype, kind) >= 0, "%s: too many tiles for one launch", who);
     for (int i = 0; i < l.problems; ++i) {
         GemmProblem &q = l.q[i];
-        q.quads = q.N % 4 == 0 && q.N < (1 << 23);  // 32 rows of 4-byte elements stay under 2^31 bytes
-        for (const void *o : {(const void *)q.out[0], (const void *)q.out[1], (const void *)q.out[2], q.in[0], q.in[1]})
-            if ((uintptr_t)o % 16) q.quads = 0;
+        q.short_rows = q.N < (1 << 23);
         q.partial = partial;
         if (q.splits > 1) partial += (long long)q.splits * (gated ? 2 : 1) * q.M * ((q.N + 3LL) / 4 * 4);
     }

@@ -58,7 +58,7 @@ struct GemmProblem {
     int M, N, K, parts;
     void *out[3];                // rows of N elements, dense; EPI_GATED: h, gate and up (float32 or null); EPI_GATED_BWD: dgate, dup
     const void *in[2];           // EPI_GATED_BWD: gate, up (float32)
-    int quads;                   // N % 4 == 0 and outputs aligned: four columns per store
+    int short_rows;              // N < 2^23: 32 rows of four-byte elements stay under 2^30 bytes
     int splits, stages_per_split;
     float *partial;
     // filled in by the launcher
