@@ -478,8 +478,11 @@ int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStrea
     const unsigned per_block = bwd ? ROT_BWD_THREADS / 64 : 4;
     unsigned blocks = (p.items + per_block - 1) / per_block;
     if (blocks > (unsigned)max_blocks) blocks = max_blocks;
-    if (W == WV && chunks <= 64) return launch_pairs<T, WV, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
-    if (W == WV / 2 && W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    // (a head of up to 512 channels: at most 64 chunks of 16 bytes or of 8 in a 16-bit type, 128 of 8 bytes in float32, 256 of one pair)
+    if (W == WV) return launch_pairs<T, WV, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    if (W > 1 && chunks <= 64) return launch_pairs<T, WV / 2, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
+    if constexpr (sizeof(T) == 4)
+        if (W > 1) return launch_pairs<T, WV / 2, 2>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
     if (chunks <= 64) return launch_pairs<T, 1, 1>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
     if (chunks <= 128) return launch_pairs<T, 1, 2>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);
     return launch_pairs<T, 1, 4>(p, mode, lp_log2, lp, (int)blocks, dw0, dw1, s);

@@ -64,6 +64,9 @@ SHAPES = [
     (3, 8191, 1, 1, 64, (24, 16, 24), "bhnd"),  # ... and several small ones
     (2, 20011, 3, 1, 16, (16,), "dense"),
     (1, 33001, 2, 2, 7, (4, 2), "packed"),
+    (2, 3, 2, 1, 260, (100, 60), "dense"),      # wide heads in whole vectors of 8 bytes, not of 16
+    (1, 5, 3, 2, 508, (508,), "packed"),
+    (1, 4, 2, 3, 300, (4, 200), "bhnd"),
 ]
 
 
