@@ -89,7 +89,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     if ((kind == GEMM_GATE_UP || kind == GEMM_DOWN) && l.direct && l.q[0].M >= 1 && l.q[0].M <= 256) {
         GemmProblem &q = l.q[0];
         const int m_tiles = (q.M + 15) / 16;
-        if (q.M <= 64 || (long long)m_tiles * (gated ? 2 : 1) * q.N * q.K * (long long)elem_size(dtype) <= (12LL << 20)) {
+        if (q.M <= 64 || (double)m_tiles * (gated ? 2 : 1) * q.N * q.K * elem_size(dtype) <= (12 << 20)) {
             l.tile = TILE_SKINNY;
             q.splits = 1;
             const long long slices = (q.N + 15) / 16;
@@ -192,9 +192,10 @@ struct FfnLaunches {
 FfnLaunches ffn_launches(const gd_ffn_desc *d, const void *x, const void *wg, const void *wu, const void *wd, const void *hidden, const void *dy,
                          long long ld_dy, const void *dgate, const void *dup) {
     const size_t es = elem_size(d->dtype);
-    const Matrix X{x, d->rows, d->in, d->ld_x}, Wg{wg, d->hidden, d->in, d->ld_w_in}, Wu{wu, d->hidden, d->in, d->ld_w_in},
-        Wd{wd, d->out, d->hidden, d->ld_w_down}, H{hidden, d->rows, d->hidden, d->hidden}, DY{dy, d->rows, d->out, ld_dy},
-        DG{dgate, d->rows, d->hidden, d->hidden}, DU{dup, d->rows, d->hidden, d->hidden};
+    auto matrix = [](const void *p, long long rows, long long cols, long long ld) { return Matrix{p, rows, cols, rows <= 1 ? cols : ld}; };
+    const Matrix X = matrix(x, d->rows, d->in, d->ld_x), Wg = matrix(wg, d->hidden, d->in, d->ld_w_in), Wu = matrix(wu, d->hidden, d->in, d->ld_w_in),
+                 Wd = matrix(wd, d->out, d->hidden, d->ld_w_down), H = matrix(hidden, d->rows, d->hidden, d->hidden),
+                 DY = matrix(dy, d->rows, d->out, ld_dy), DG = matrix(dgate, d->rows, d->hidden, d->hidden), DU = matrix(dup, d->rows, d->hidden, d->hidden);
     FfnLaunches f{};
     for (auto &l : f.l) { l.problems = 1; l.direct = !d->unaligned; l.act = d->act; }
     const Matrix w_in[2] = {Wg, Wu}, d_in[2] = {DG, DU};
@@ -227,10 +228,13 @@ long long partial_floats(FfnLaunches f, int dtype, int first, int last) {
     return most;
 }
 
-int check_as_sized(const FfnLaunches &f, const gd_ffn_desc *d, int first, int last, const char *who) {
+// The launches take the path that the workspace was sized for.  Rows of dy may be aligned where dense ones, which that takes for granted, are not
+int as_sized(FfnLaunches &f, const gd_ffn_desc *d, int first, int last, const char *who) {
     const FfnLaunches sized = ffn_sizing(d);
-    for (int k = first; k <= last; ++k)
-        GD_CHECK(f.l[k].direct == sized.l[k].direct, "%s: a tensor does not start (or rows of dy are not apart by) a multiple of 16 bytes: set unaligned", who);
+    for (int k = first; k <= last; ++k) {
+        GD_CHECK(f.l[k].direct || !sized.l[k].direct, "%s: a tensor does not start (or rows of dy are not apart by) a multiple of 16 bytes: set unaligned", who);
+        f.l[k].direct = sized.l[k].direct;
+    }
     return 0;
 }
 
@@ -257,7 +261,7 @@ int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const 
     GD_CHECK((uintptr_t)workspace_dev % 16 == 0, "%s: workspace not aligned to 16 bytes", who);
     GD_CHECK(workspace_dev || gd_gated_ffn_workspace(d, 0) == 0, "%s: null workspace", who);
     FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden_dev, nullptr, d->out, nullptr, nullptr);
-    GD_TRY(check_as_sized(f, d, GEMM_GATE_UP, GEMM_DOWN, who));
+    GD_TRY(as_sized(f, d, GEMM_GATE_UP, GEMM_DOWN, who));
     GemmLaunch &g = f.l[GEMM_GATE_UP], &o = f.l[GEMM_DOWN];
     g.q[0].out[0] = hidden_dev; g.q[0].out[1] = gate_dev; g.q[0].out[2] = up_dev;
     o.q[0].out[0] = y;
@@ -279,7 +283,7 @@ int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy,
     void *dgate = ws, *dup = ws ? ws + grad : nullptr;
     float *partial = reinterpret_cast<float *>(ws ? ws + 2 * grad : nullptr);
     FfnLaunches f = ffn_launches(d, x, w_gate, w_up, w_down, hidden, dy, ld_dy, dgate, dup);
-    GD_TRY(check_as_sized(f, d, empty ? GEMM_DW : GEMM_DHIDDEN, GEMM_DW, who));
+    GD_TRY(as_sized(f, d, empty ? GEMM_DW : GEMM_DHIDDEN, GEMM_DW, who));
     hipStream_t s = (hipStream_t)stream;
     if (!empty) {
         GemmProblem &h = f.l[GEMM_DHIDDEN].q[0];

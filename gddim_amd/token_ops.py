@@ -263,8 +263,10 @@ def _check_ffn(x, w_gate, w_up, w_down, act):
         raise GddimError("x %s, w_gate %s, w_up %s, w_down %s do not fit (..., in), (hidden, in), (hidden, in), (out, hidden)" % (xs, gs, us, ds))
     x, w_gate, w_up, w_down = _rows(x, gs[1]), _rows(w_gate, gs[1]), _rows(w_up, gs[1]), _rows(w_down, gs[0])
     ld = w_gate.stride(0)
-    if ld != w_up.stride(0):
-        w_gate, w_up, ld = w_gate.contiguous(), w_up.contiguous(), gs[1]
+    if ld != w_up.stride(0):  # (of a single row: never used)
+        if gs[0] > 1:
+            w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+        ld = gs[1]
     rows = x.shape[0]
     if rows > 1 << 30 or gs[0] > 1 << 30 or gs[1] > 1 << 30 or ds[0] > 1 << 30:
         raise GddimError("sizes past 2^30: %d rows, %d -> %d -> %d" % (rows, gs[1], gs[0], ds[0]))
@@ -328,7 +330,8 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
             raise GddimError("saved %s has shape %s, expected (%d, %d), dense" % (name, tuple(t.shape), M, F))
     dy = _rows(dy, O)
     gate, up, hidden = saved
-    if (dy.data_ptr() | gate.data_ptr() | up.data_ptr() | hidden.data_ptr()) & 15 or (dy.stride(0) != O and dy.stride(0) * dy.element_size() % 16):
+    apart = dy.stride(0) * dy.element_size() if M > 1 else 0  # rows of dy: within what the aligned path takes, where dense ones would be
+    if (dy.data_ptr() | gate.data_ptr() | up.data_ptr() | hidden.data_ptr()) & 15 or (dy.stride(0) != O and (apart % 16 or apart > 1 << 22)):
         fields = fields[:6] + (1,) + fields[7:]
     dx, dwg, dwu, dwd = x.new_empty((M, D)), x.new_empty((F, D)), x.new_empty((F, D)), x.new_empty((O, F))
     ws, ws_at = _workspace(x, fields, 1)

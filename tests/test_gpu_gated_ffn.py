@@ -215,6 +215,38 @@ def test_strides_and_batches(dev, typ):
     _check(ops.gated_ffn(one, wg, wu, wd, act="gelu"), ref.gated_ffn(one, wg, wu, wd, "gelu", dtype), "expanded")
 
 
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+@pytest.mark.parametrize("size,apart", [((70, 64, 72, 100), 104), ((70, 64, 72, 98), 104), ((300, 40, 264, 13), 16), ((70, 64, 72, 96), 99), ((70, 63, 72, 96), 104), ((3, 64, 72, 96), (1 << 21) + 8)], ids=str)
+def test_rows_of_dy_apart(dev, size, apart, typ):
+    """dense rows of dy would not be aligned, these are; and the other way round"""
+    from gddim_amd import ops
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ], 7)
+    wide = torch.full((size[0], apart), 7.0, dtype=TYPES[typ], device=dev)
+    wide[:, :size[3]] = dy
+    want = _run(x, wg, wu, wd, dy, "silu")
+    got = _run(x, wg, wu, wd, wide[:, :size[3]], "silu")
+    for g, w, f64, what in zip(got, want, ref.gated_ffn(x, wg, wu, wd, "silu", TYPES[typ], dy), ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, f64, what)
+        _check(w, f64, what)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f32"])
+@pytest.mark.parametrize("apart", [0, 1, 24, 1 << 40])
+def test_row_stride_of_a_single_row_means_nothing(dev, apart, typ):
+    size = (1, 64, 72, 40)
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ], 8)
+    x[0, 5] = float("inf")  # padded rows of the sums over rows must not meet it
+    wg[:, 5] = wg[:, 5].abs() * 1e-3
+    want = _run(x, wg, wu, wd, dy, "silu")
+    for g, w in zip(_run(x.as_strided((1, 64), (apart, 1)), wg, wu, wd, dy.as_strided((1, 40), (apart, 1)), "silu"), want):
+        assert torch.equal(g.nan_to_num(123.0), w.nan_to_num(123.0))
+    one = _inputs(dev, 5, 64, 1, 1, TYPES[typ], 8)  # weights of one row
+    want = _run(*one, "gelu")
+    w = [t.as_strided(t.shape, (apart + i, 1)) for i, t in enumerate(one[1:4])]
+    for g, v in zip(_run(one[0], *w, one[4], "gelu"), want):
+        assert torch.equal(g, v)
+
+
 @pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("M", [1, 7, 40, 200])
 def test_infinities_and_nan_stay_in_their_row(dev, typ, M):
