@@ -86,14 +86,20 @@ class RotaryAxes:
         device = torch.device("cuda") if device is None else torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.frequencies = torch.as_tensor(frequencies, dtype=torch.float64).detach().to(device).clone(memory_format=torch.contiguous_format)
-        if tuple(self.frequencies.shape) != (sum(self.sections) // 2,):
-            raise GddimError("RotaryAxes: frequencies of shape %s, expected (%d,)" % (tuple(self.frequencies.shape), sum(self.sections) // 2))
+        # from a table of its own in host memory: the copy has ended when this returns, so that any stream may use it
+        self._frequencies = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu().clone(memory_format=torch.contiguous_format).to(device)
+        if tuple(self._frequencies.shape) != (sum(self.sections) // 2,):
+            raise GddimError("RotaryAxes: frequencies of shape %s, expected (%d,)" % (tuple(self._frequencies.shape), sum(self.sections) // 2))
         self.device = device
         self._rotated = sum(self.sections)
         self._index = device.index if device.type == "cuda" else -1
         self._halves = int(paired == "halves")
         self._section = self.sections + (0,) * (_abi.GD_MAX_AXES - len(self.sections))
+
+    @property
+    def frequencies(self):
+        """radians per unit of position, (sum(sections) / 2,) float64"""
+        return self._frequencies
 
 
 def _heads(t):
@@ -157,7 +163,7 @@ def _rotary_desc(x, pos, axes):
         raise GddimError("sections %r of %d channels exceed the head's %d" % (axes.sections, axes._rotated, D))
     if B * N >= 1 << 31:
         raise GddimError("%d x %d tokens do not fit 31 bits" % (B, N))
-    return _ROTARY.pack(types[x.dtype], B, N, D, A, *axes._section, axes._halves, kind, pos.data_ptr(), sb, sn, sa, axes.frequencies.data_ptr())
+    return _ROTARY.pack(types[x.dtype], B, N, D, A, *axes._section, axes._halves, kind, pos.data_ptr(), sb, sn, sa, axes._frequencies.data_ptr())
 
 
 def rotary(x, pos, axes, inverse=False):

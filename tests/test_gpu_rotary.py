@@ -310,3 +310,22 @@ def test_refusals_on_the_gpu(dev):
             pytest.fail("call %d was not refused" % i)
     with torch.no_grad():
         ops.rotary(x, pos, axes)
+
+
+def test_axes_are_ready_for_any_stream(dev):
+    """a table made while its stream is busy, used on another one at once"""
+    from gddim_amd import ops
+    g = _gen(77)
+    x, pos = torch.randn(1, 65, 2, 16, generator=g).to(dev), torch.randint(-99, 99, (65, 1), generator=g).to(dev)
+    freq = torch.rand(8, dtype=torch.float64, generator=g)
+    want = ops.rotary(x, pos, ops.RotaryAxes((16,), frequencies=freq, device=dev))
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device=dev)
+    for _ in range(20):
+        busy = torch.mm(busy, busy) * 1e-3
+    axes = ops.RotaryAxes((16,), frequencies=freq.to(dev), device=dev)
+    with torch.cuda.stream(other):
+        got = ops.rotary(x, pos, axes)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

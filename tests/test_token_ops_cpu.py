@@ -180,3 +180,5 @@ def test_rotary_axes_copies(native_lib):
     assert axes.frequencies.tolist() == [1.0, 1.0]
     other = copy.deepcopy(axes)
     assert other.frequencies.data_ptr() != axes.frequencies.data_ptr() and other.sections == axes.sections
+    with pytest.raises(AttributeError):  # a kernel reads as many of them as the sections say
+        axes.frequencies = torch.ones(1)
