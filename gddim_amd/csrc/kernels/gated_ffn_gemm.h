@@ -9,17 +9,20 @@
 // C[m][n] = sum_k A[m][k] B[n][k].  Each operand lies in memory with k adjacent (KC: x, weights as torch.nn.Linear keeps them) or with its other index
 // adjacent (the weights in dh and dx, everything in the weights' gradients); no operand is transposed in memory.
 //
-// Tiles.  A step of the k loop takes 64 bytes of k (32 16-bit or 16 float32 values) of BM rows of A and BN of B.  A fragment is 16 bytes a lane: row
-// (lane % 16) and k = 8 (lane / 16) .. + 7 of a 16-row x 32-k block (16-bit types; the transposing LDS read gathers it where k is not adjacent), one
-// v_mfma_f32_16x16x32; in float32 four values, four v_mfma_f32_16x16x4.  A sum does not care which k a lane holds as long as both operands agree, so
-// both layouts and all types share one loop.  The MFMA's first operand is B: a lane then ends with four ADJACENT n of one row m.
-// A stage is two steps, 128 bytes of k: KC rows take whole lines (with 64-byte rows the requests to L2 doubled and became the bound: y of 16384 x 1024 x
-// 4096 in 153 us instead of 129), 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  No bank conflicts
-// either way (counted).  Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows
-// are not whole 16-byte pieces, through registers.
+// Tiles.  A stage is 128 bytes of k (64 16-bit or 32 float32 values) of BM rows of A and BN of B, a step a quarter of it.  A fragment is 16 bytes a lane: row
+// (lane % 32) and k = 8 (lane / 32) .. + 7 of a 32-row x 16-k block (16-bit types; the transposing LDS read gathers it where k is not adjacent), one
+// v_mfma_f32_32x32x16; in float32 four values, four v_mfma_f32_32x32x2.  A sum does not care which k a lane holds as long as both operands agree, so
+// both layouts and all types share one loop.  The MFMA's first operand is B: a lane then ends with groups of four ADJACENT n of one row m.
+// In LDS a KC row is one line of 128 bytes (with stages of 64 bytes the requests to L2 doubled and became the bound: y of 16384 x 1024 x 4096 in 153 us
+// instead of 129), 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  No bank conflicts either way (counted).
+// Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole
+// 16-byte pieces, through registers.
 // Two stages lie in LDS.  A step multiplies fragments that were read during the step before, those of the next are read between its products: when a stage's
-// second step begins all of it has been read, and the stage after the next is requested into its place, two steps (2048 MFMA cycles of a 256 x 256
-// tile) before it is needed.
+// last step begins all of it has been read, and the stage after the next is requested into its place, a whole stage (2048 MFMA cycles a SIMD of a 256 x
+// 256 tile) before it is needed.
+//
+// What bounds them: with k long, the matrix core at the clock that the card's power leaves it (1.64 to 1.75 GHz in bf16: 16384 x 1024 x 4096, products of 137
+// to 412 GFLOP, at 0.95 to 1.17 PFLOP/s; a library product of these shapes reaches 0.91 to 1.38), in float32 its rate (133 to 138 TFLOP/s; library 138 to 150).
 //
 // All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type are only operands of a next product, as the 16-bit matrix core
 // wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients at
@@ -192,9 +195,9 @@ struct Operand {
     static constexpr int BYTES = R * 128;
 
     // A piece's slot in the stage: (i * WAVES + wave) * 64 + lane, slot / CPR its row (KC: of the matrix tile; else of k).  Its first row is the same for a wave's 64
-    // slots, and the swizzle of row i repeats every PERIOD i: a lane keeps PERIOD offsets, the rest of an address is the wave's.
-    static constexpr int RPI = 64 / CPR, PERIOD = 1;
-    static_assert(PIECES % PERIOD == 0 && (KC ? WAVES * RPI % 16 == 0 : ES == 2 ? WAVES * RPI % 4 == 0 : WAVES * RPI % 8 == 0), "");
+    // slots, and the swizzle of a lane's row is the same for every i: a lane keeps one offset, the rest of an address is the wave's.
+    static constexpr int RPI = 64 / CPR;
+    static_assert(KC ? WAVES * RPI % 16 == 0 : ES == 2 ? WAVES * RPI % 4 == 0 : WAVES * RPI % 8 == 0, "");
 
     const char *base[2];   // element (first row, k = 0) of each source
     long long end;         // bytes from there to the end of the matrix
@@ -203,7 +206,7 @@ struct Operand {
     int rows_left;         // rows (KC) / columns (else) from the tile's first
 
     __device__ static __forceinline__ int row_of(int i, int wave, int lane) { return (i * WAVES + wave) * RPI + lane / CPR; }
-    __device__ static __forceinline__ int piece_of(int i, int wave, int lane) { return lane % CPR ^ swizzle(row_of(i % PERIOD, wave, lane)); }
+    __device__ static __forceinline__ int piece_of(int wave, int lane) { return lane % CPR ^ swizzle(row_of(0, wave, lane)); }
     __device__ static __forceinline__ int swizzle(int r) {
         if constexpr (KC) return kc_swizzle(r);
         else if constexpr (ES == 2) return 4 * (r & 3);  // four k rows of 64 bytes on different banks
@@ -219,7 +222,7 @@ struct Operand {
     static_assert(!GATED_B || WAVES == 4 || WAVES == 8, "");
     struct Request {
         i32x4 buffer[BUFFERS];
-        unsigned off[PERIOD];
+        unsigned off;
     };
     // stage st (src: which source of a two-part sum)
     __device__ __forceinline__ Request request(int src, int st, bool any, int wave, int lane) const {
@@ -229,23 +232,20 @@ struct Operand {
         Request r;
 #pragma unroll
         for (int g = 0; g < BUFFERS; ++g) r.buffer[g] = buffer_of(base[!GATED_B ? src : BUFFERS == 2 ? g : wave >> 2] + adv, (int)left);
-#pragma unroll
-        for (int t = 0; t < PERIOD; ++t) {
-            r.off[t] = (unsigned)(lane / CPR) * (unsigned)ld + piece_of(t, wave, lane) * 16;
-            if (KC && st * KSTAGE + piece_of(t, wave, lane) * V >= k_len) r.off[t] = OUT_OF_RANGE;
-        }
+        r.off = (unsigned)(lane / CPR) * (unsigned)ld + piece_of(wave, lane) * 16;
+        if (KC && st * KSTAGE + piece_of(wave, lane) * V >= k_len) r.off = OUT_OF_RANGE;
         return r;
     }
     // its i-th piece straight into LDS
     __device__ __forceinline__ void issue(const Request &r, int i, char *lds, int wave) const {
         const int row = (i * WAVES + wave) * RPI;
-        load_to_lds(r.buffer[BUFFERS == 2 ? i & 1 : 0], r.off[i % PERIOD] + (unsigned)row_in_source(row) * (unsigned)ld, lds + (i * WAVES + wave) * 1024);
+        load_to_lds(r.buffer[BUFFERS == 2 ? i & 1 : 0], r.off + (unsigned)row_in_source(row) * (unsigned)ld, lds + (i * WAVES + wave) * 1024);
     }
     // ... through registers, for rows that are not whole aligned pieces
     __device__ __forceinline__ void load_regs(i32x4 *r, int src, int st, int wave, int lane) const {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int row = row_of(i, wave, lane), piece = piece_of(i, wave, lane);
+            const int row = row_of(i, wave, lane), piece = piece_of(wave, lane);
             const int k0 = st * KSTAGE + (KC ? piece * V : row);
             const int s = GATED_B ? source_of(row) : src;
             const int rr = KC ? row_in_source(row) : piece * V;  // first row / column
@@ -307,7 +307,8 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // 32 rows of accumulators from LDS through the epilogue.  Inside the matrix (all of a large one) the loop is stripped of bounds, of 64-bit
-// address arithmetic and of the choice of activation: with those, instructions bound it (13 us of a tile's 43 at 16384 x 1024 x 4096).
+// address arithmetic and of the choice of activation.  Row by row through LDS, because accumulators that met the epilogue in place went to scratch
+// memory (dhidden of 16384 x 1024 x 4096 977 us instead of 284).
 template <typename T, int EPI, int ACT>
 __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mine, int m, int n, int lane) {
     constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p
     constexpr bool GATED = EPI == EPI_GATED;
     constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
     static_assert(TN == 64 && TM % 32 == 0, "a wave's 64 columns (32 of gate and 32 of up) and groups of 32 rows go through 8 KB of LDS");
-        typedef Operand<T, BM, AKC, THREADS, false> OpA;
+    typedef Operand<T, BM, AKC, THREADS, false> OpA;
     typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
     constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES, KSTAGE = OpA::KSTAGE;
     static_assert(WM * WN * 8192 == STAGE, "the epilogue takes one place, the next piece's first stage the other");
