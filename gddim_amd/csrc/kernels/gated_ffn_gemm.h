@@ -416,8 +416,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p
     typedef Operand<T, BM, AKC, THREADS, false> OpA;
     typedef Operand<T, BN, BKC, THREADS, GATED> OpB;
     constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES, KSTAGE = OpA::KSTAGE;
-    static_assert(WM * WN * 8192 == STAGE, "the epilogue takes one place, the next piece's first stage the other");
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+    constexpr int PLACE = STAGE > WM * WN * 8192 ? STAGE : WM * WN * 8192;  // the epilogue takes one place, the next piece's first stage the other
+    __shared__ __attribute__((aligned(16))) char lds[2 * PLACE];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p
     };
 
     int at = 0;  // place of the current piece's stage 0
-    auto place_of = [&](int st) __attribute__((always_inline)) { return lds + ((at + st) & 1) * STAGE; };
+    auto place_of = [&](int st) __attribute__((always_inline)) { return lds + ((at + st) & 1) * PLACE; };
     i32x4 ra[DIRECT ? 1 : OpA::PIECES], rb[DIRECT ? 1 : OpB::PIECES];
     // stage st of the open piece: what its requests share, then its LOADS requests one by one (or, through registers, all of it)
     typename OpA::Request qa;
@@ -726,6 +726,11 @@ int launch_gemm(const GemmLaunch &p, hipStream_t s) {
     if (p.blocks > 0) {
         if (p.tile == TILE_256) {
             if constexpr (sizeof(T) == 2) gemm_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, true><<<p.grid, 512, 0, s>>>(p);
+        } else if (p.tile == TILE_NARROW) {
+            if constexpr (sizeof(T) == 4) {
+                if (p.direct) gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
+                else gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
+            }
         } else if (p.direct) gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
         else gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
         GD_HIP(hipGetLastError());

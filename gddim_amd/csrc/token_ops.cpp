@@ -107,48 +107,58 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
         }
     }
     const int kstage = 128 / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
-    auto tiles_n = [&](const GemmProblem &q, int t) { const int n = gated ? t / 2 : t; return (q.N + n - 1LL) / n; };
+    struct Shape { GemmTile tile; int m, n; };
+    const Shape shapes[3] = {{TILE_128, 128, 128}, {TILE_256, 256, 256}, {TILE_NARROW, 128, 64}};
+    auto tiles_n = [&](const GemmProblem &q, int bn) { const int n = gated ? bn / 2 : bn; return (q.N + n - 1LL) / n; };
     auto stages_of = [&](const GemmProblem &q) { return q.K ? (long long)q.parts * ((q.K + kstage - 1) / kstage) : 1; };
-    // Tile and split of the sums by estimated time, in us.  A 256 x 256 tile holds a CU, 128 x 128 ones share it by two or more; a CU with c tiles takes c times a
+    // Tile and split of the sums by estimated time, in us.  A 256 x 256 tile holds a CU, smaller ones share it by two or more; a CU with c tiles takes c times a
     // stage's time per stage, and a fixed time for the way in and out.  Split sums are written and read again by the join.  The constants are fits to y
     // = h Wd^T of 16384 x 1024, K = 256 .. 4096, in bf16 (256: 16.5, 23.6, 36.8, 127.9 us; 128: 18.4, 25.6, 40.5, 148.9) and to one and two 128 tiles a CU
-    // (21.6, 24.9 us at K = 1024; in float32 2.3 and 1.8 us a stage and tile); operands whose k is not adjacent cost the small tile more (the weights'
-    // gradients of 16384 x 1024 x 4096: 432 us with 256, 554 with 128), and where every CU multiplies, the clock falls: split four ways over all of them these
-    // gradients' 192 tiles take 421 us and the join 45.
+    // (21.6, 24.9 us at K = 1024); operands whose k is not adjacent cost the small tile more (the weights' gradients of 16384 x 1024 x 4096: 432 us with 256,
+    // 554 with 128), and where every CU multiplies, the clock falls: split four ways over all of them these gradients' 192 tiles take 421 us and the join 45.
+    // In float32 the matrix core is 16 times slower, so tiles of 128 x 64 cost little per product (8192 x 1024 x 4096: gate and up 1.12 ms, 1.03 with 128 x 128)
+    // and fill narrow matrices and the last round of tiles better (6080 x 192 x 2464: down 81 -> 71 us, dx 150 -> 120, the weights' gradients 224 -> 199; gate and
+    // up of 4096 x 256 x 684 44 -> 37.5; dhidden, whose single tile on a CU waits for the projections it reads and the gradients it writes, 37 -> 30).
     const double stage128 = kind == GEMM_DW ? 0.72 : kind == GEMM_DHIDDEN || kind == GEMM_DX ? 0.65 : 0.57;
     const long long stages = stages_of(l.q[0]);
     double best = 1e30;
     long long best_split = 1;
-    for (int t = 128; t <= 256; t += 128) {
-        if (t == 256 && (dtype == GD_F32 || !l.direct)) continue;
+    Shape chosen = shapes[0];
+    for (const Shape &t : shapes) {
+        if (t.tile == TILE_256 && (dtype == GD_F32 || !l.direct)) continue;
+        if (t.tile == TILE_NARROW && dtype != GD_F32) continue;
         long long n = 0;
         double out = 0;
         for (int i = 0; i < l.problems; ++i) {
-            n += ((l.q[i].M + t - 1LL) / t) * tiles_n(l.q[i], t);
+            n += ((l.q[i].M + t.m - 1LL) / t.m) * tiles_n(l.q[i], t.n);
             out += (double)l.q[i].M * l.q[i].N * (gated ? 2 : 1);
         }
         if (n > (1LL << 30)) return -1;
         for (long long s = 1; s <= 16 && s <= stages && (s == 1 || stages / s >= 4); ++s) {
             const double per = (double)((stages + s - 1) / s), c = (double)((n * s + cus - 1) / cus);
             double us;
-            if (t == 256) us = c * ((kind != GEMM_DW ? 1.9 : n * s < cus ? 1.7 : 2.1) * per + 3) + 5;
-            else if (dtype == GD_F32) us = c <= 1 ? 2.3 * per + 5 : 1.8 * c * per + 8;
+            if (t.tile == TILE_256) us = c * ((kind != GEMM_DW ? 1.9 : n * s < cus ? 1.7 : 2.1) * per + 3) + 5;
+            else if (dtype == GD_F32) {
+                const bool narrow = t.tile == TILE_NARROW;
+                us = c <= 1 ? (narrow ? 1.45 : 2.45) * per + 5 : (narrow ? 1.09 : 2.0) * c * per + 8;
+                if (kind == GEMM_DHIDDEN && c <= 1) us += out * 16 / 4.5e6;
+            }
             else us = c <= 1 ? 1.05 * per + 5 : stage128 * c * per + 8;
             if (s > 1) us += 4 + (double)s * out * 8 / 4.5e6;
             if (us < best) {
                 best = us;
                 best_split = s;
-                l.tile = t == 256 ? TILE_256 : TILE_128;
+                chosen = t;
             }
         }
     }
-    const int t = l.tile == TILE_256 ? 256 : 128;
+    l.tile = chosen.tile;
     const long long room = l.tile == TILE_256 ? cus : 2 * cus;
     long long floats = 0, join = 0, blocks = 0;
     for (int i = 0; i < l.problems; ++i) {
         GemmProblem &q = l.q[i];
-        q.tiles_m = (int)((q.M + t - 1LL) / t);
-        q.tiles_n = (int)tiles_n(q, t);
+        q.tiles_m = (int)((q.M + chosen.m - 1LL) / chosen.m);
+        q.tiles_n = (int)tiles_n(q, chosen.n);
         q.stages_per_split = (int)((stages_of(q) + best_split - 1) / best_split);
         q.splits = (int)((stages_of(q) + q.stages_per_split - 1) / q.stages_per_split);
         q.blocks = q.tiles_m * q.tiles_n * q.splits;

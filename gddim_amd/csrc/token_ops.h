@@ -48,7 +48,7 @@ int launch_rotary(RotaryParams p, int dtype, RotaryMode mode, void *dw0, void *d
 // ---- gated feed-forward block (kernels/gated_ffn_gemm.h) ----
 enum GemmKind { GEMM_GATE_UP, GEMM_DOWN, GEMM_DHIDDEN, GEMM_DX, GEMM_DW };
 enum GemmEpilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD };
-enum GemmTile { TILE_128, TILE_256, TILE_SKINNY };
+enum GemmTile { TILE_128, TILE_256, TILE_NARROW, TILE_SKINNY };  // NARROW: 128 x 64
 
 // C[m][n] = sum over parts and k of A[m][k] B[n][k]
 struct GemmProblem {
