@@ -209,7 +209,7 @@ struct Operand {
     __device__ static __forceinline__ int piece_of(int wave, int lane) { return lane % CPR ^ swizzle(row_of(0, wave, lane)); }
     __device__ static __forceinline__ int swizzle(int r) {
         if constexpr (KC) return kc_swizzle(r);
-        else if constexpr (ES == 2) return 4 * (r & 3);  // four k rows of 64 bytes on different banks
+        else if constexpr (ES == 2) return R == 64 ? 2 * (r & 2) : 4 * (r & 3);  // four k rows of 64 bytes on different banks
         else return 8 * ((r >> 2) & 1);
     }
     // gated B tiles: rows of gate and up alternate in blocks of 32, so that a wave's 64 columns hold both of its 32
@@ -727,10 +727,8 @@ int launch_gemm(const GemmLaunch &p, hipStream_t s) {
         if (p.tile == TILE_256) {
             if constexpr (sizeof(T) == 2) gemm_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, true><<<p.grid, 512, 0, s>>>(p);
         } else if (p.tile == TILE_NARROW) {
-            if constexpr (sizeof(T) == 4) {
-                if (p.direct) gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
-                else gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
-            }
+            if (p.direct) gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
+            else gemm_kernel<T, 128, 64, 4, 1, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
         } else if (p.direct) gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, true><<<p.grid, 256, 0, s>>>(p);
         else gemm_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, false><<<p.grid, 256, 0, s>>>(p);
         GD_HIP(hipGetLastError());

@@ -116,17 +116,21 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     // = h Wd^T of 16384 x 1024, K = 256 .. 4096, in bf16 (256: 16.5, 23.6, 36.8, 127.9 us; 128: 18.4, 25.6, 40.5, 148.9) and to one and two 128 tiles a CU
     // (21.6, 24.9 us at K = 1024); operands whose k is not adjacent cost the small tile more (the weights' gradients of 16384 x 1024 x 4096: 432 us with 256,
     // 554 with 128), and where every CU multiplies, the clock falls: split four ways over all of them these gradients' 192 tiles take 421 us and the join 45.
-    // In float32 the matrix core is 16 times slower, so tiles of 128 x 64 cost little per product (8192 x 1024 x 4096: gate and up 1.12 ms, 1.03 with 128 x 128)
-    // and fill narrow matrices and the last round of tiles better (6080 x 192 x 2464: down 81 -> 71 us, dx 150 -> 120, the weights' gradients 224 -> 199; gate and
-    // up of 4096 x 256 x 684 44 -> 37.5; dhidden, whose single tile on a CU waits for the projections it reads and the gradients it writes, 37 -> 30).
-    const double stage128 = kind == GEMM_DW ? 0.72 : kind == GEMM_DHIDDEN || kind == GEMM_DX ? 0.65 : 0.57;
+    // Tiles of 128 x 64 cost more per product but fill narrow matrices and the last round of tiles better.  float32, whose matrix core is 16 times slower: 8192
+    // x 1024 x 4096 gate and up 1.12 ms (1.03 with 128 x 128), 6080 x 192 x 2464 down 71 us (81), dx 120 (150), the weights' gradients 199 (224); gate and up of
+    // 4096 x 256 x 684 37.5 (44).  bf16: 2048 x 1024 x 4096 down 32 us (27), 10069 x 344 x 1208 24 (28), dhidden 49 (54, with 256), of 658 x 184 x 2712 14 (18):
+    // each tile of dhidden waits for the projections it reads, once for every 32 rows of a wave (one, two or four times in a tile).  Through registers a stage takes about twice as long
+    // (428 x 884 x 2764 in fp16: dhidden 28 us, 43 with 128 x 128; dx 22, 29).
+    struct Cost { double alone, shared; };  // us a stage and tile
+    const bool f32 = dtype == GD_F32, dhidden = kind == GEMM_DHIDDEN;
+    const Cost wide = f32 ? Cost{2.45, 2.0} : Cost{1.05, kind == GEMM_DW ? 0.72 : dhidden || kind == GEMM_DX ? 0.65 : 0.57};
+    const Cost narrow = f32 ? Cost{1.45, 1.09} : Cost{0.85, kind == GEMM_DW ? 0.45 : dhidden ? 0.53 : 0.43};
     const long long stages = stages_of(l.q[0]);
     double best = 1e30;
     long long best_split = 1;
     Shape chosen = shapes[0];
     for (const Shape &t : shapes) {
         if (t.tile == TILE_256 && (dtype == GD_F32 || !l.direct)) continue;
-        if (t.tile == TILE_NARROW && dtype != GD_F32) continue;
         long long n = 0;
         double out = 0;
         for (int i = 0; i < l.problems; ++i) {
@@ -138,12 +142,13 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
             const double per = (double)((stages + s - 1) / s), c = (double)((n * s + cus - 1) / cus);
             double us;
             if (t.tile == TILE_256) us = c * ((kind != GEMM_DW ? 1.9 : n * s < cus ? 1.7 : 2.1) * per + 3) + 5;
-            else if (dtype == GD_F32) {
-                const bool narrow = t.tile == TILE_NARROW;
-                us = c <= 1 ? (narrow ? 1.45 : 2.45) * per + 5 : (narrow ? 1.09 : 2.0) * c * per + 8;
-                if (kind == GEMM_DHIDDEN && c <= 1) us += out * 16 / 4.5e6;
+            else {
+                const Cost &k = t.tile == TILE_NARROW ? narrow : wide;
+                us = c <= 1 ? k.alone * per + 5 : k.shared * c * per + 8;
+                if (!f32 && !l.direct) us += (t.tile == TILE_NARROW ? 0.7 : 1.1) * (c <= 1 ? k.alone : k.shared * c) * per;
             }
-            else us = c <= 1 ? 1.05 * per + 5 : stage128 * c * per + 8;
+            if (dhidden && f32) us += c <= 1 ? out * 16 / 4.5e6 : 0;
+            else if (dhidden) us += out * 12 / 7e6 / (t.tile == TILE_256 ? c : c > 2 ? c / 2 : 1) + (t.tile == TILE_256 ? 16 : t.tile == TILE_128 ? 8 : 4);
             if (s > 1) us += 4 + (double)s * out * 8 / 4.5e6;
             if (us < best) {
                 best = us;

@@ -79,6 +79,19 @@ def test_tiles_that_fill_the_chip(dev, size, typ):
         _check(g, w, what)
 
 
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [(2048, 1024, 2048, 1024), (2100, 1001, 2003, 999), (429, 884, 2764, 188), (3133, 328, 280, 328), (1500, 80, 291, 80)], ids=str)
+def test_tiles_of_each_width(dev, size, typ):
+    """square matrices and narrow ones, aligned and not"""
+    x, wg, wu, wd, dy = _inputs(dev, *size, TYPES[typ], 6)
+    want = ref.gated_ffn(x, wg, wu, wd, "gelu", TYPES[typ], dy)
+    got = _run(x, wg, wu, wd, dy, "gelu")
+    for g, w, what in zip(got, want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+    for a, b in zip(got, _run(x, wg, wu, wd, dy, "gelu")):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("typ", ["bf16", "f32"])
 @pytest.mark.parametrize("size", [(8200, 64, 2600, 64), (8200, 72, 2600, 72), (8200, 200, 1304, 1304), (8200, 65, 1301, 67), (16000, 24, 2056, 24)], ids=str)
 def test_more_tiles_than_workgroups(dev, size, typ):
