@@ -119,12 +119,12 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     // Tiles of 128 x 64 cost more per product but fill narrow matrices and the last round of tiles better.  float32, whose matrix core is 16 times slower: 8192
     // x 1024 x 4096 gate and up 1.12 ms (1.03 with 128 x 128), 6080 x 192 x 2464 down 71 us (81), dx 120 (150), the weights' gradients 199 (224); gate and up of
     // 4096 x 256 x 684 37.5 (44).  bf16: 2048 x 1024 x 4096 down 32 us (27), 10069 x 344 x 1208 24 (28), dhidden 49 (54, with 256), of 658 x 184 x 2712 14 (18):
-    // each tile of dhidden waits for the projections it reads, once for every 32 rows of a wave (one, two or four times in a tile).  Through registers a stage takes about twice as long
+    // each tile of dhidden waits for the projections it reads, once for every 32 rows of a wave (one, two or four times in a tile).  Through registers a stage takes two to three times as long
     // (428 x 884 x 2764 in fp16: dhidden 28 us, 43 with 128 x 128; dx 22, 29).
     struct Cost { double alone, shared; };  // us a stage and tile
     const bool f32 = dtype == GD_F32, dhidden = kind == GEMM_DHIDDEN;
-    const Cost wide = f32 ? Cost{2.45, 2.0} : Cost{1.05, kind == GEMM_DW ? 0.72 : dhidden || kind == GEMM_DX ? 0.65 : 0.57};
-    const Cost narrow = f32 ? Cost{1.45, 1.09} : Cost{0.85, kind == GEMM_DW ? 0.45 : dhidden ? 0.53 : 0.43};
+    const Cost wide = f32 ? Cost{2.45, 2.0} : Cost{1.05, kind == GEMM_DW ? 0.6 : dhidden || kind == GEMM_DX ? 0.65 : 0.57};
+    const Cost narrow = f32 ? Cost{1.45, 1.09} : Cost{0.85, kind == GEMM_DW ? 0.5 : dhidden ? 0.53 : 0.43};
     const long long stages = stages_of(l.q[0]);
     double best = 1e30;
     long long best_split = 1;
@@ -145,7 +145,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
             else {
                 const Cost &k = t.tile == TILE_NARROW ? narrow : wide;
                 us = c <= 1 ? k.alone * per + 5 : k.shared * c * per + 8;
-                if (!f32 && !l.direct) us += (t.tile == TILE_NARROW ? 0.7 : 1.1) * (c <= 1 ? k.alone : k.shared * c) * per;
+                if (!f32 && !l.direct) us += (kind == GEMM_DW ? 1.5 : t.tile == TILE_NARROW ? 0.7 : 1.1) * (c <= 1 ? k.alone : k.shared * c) * per;
             }
             if (dhidden && f32) us += c <= 1 ? out * 16 / 4.5e6 : 0;
             else if (dhidden) us += out * 12 / 7e6 / (t.tile == TILE_256 ? c : c > 2 ? c / 2 : 1) + (t.tile == TILE_256 ? 16 : t.tile == TILE_128 ? 8 : 4);
