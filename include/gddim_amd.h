@@ -395,7 +395,7 @@ int gd_qk_norm_rotary_backward(const gd_rotary_desc *d, const gd_heads *dq_out, 
                                float eps, void *workspace_dev, void *dw_q, void *dw_k, void *stream);
 /* Gated feed-forward block on `rows` tokens:  y = (act(x w_gate^T) (.) (x w_up^T)) w_down^T,  x (rows, in), w_gate and w_up (hidden, in),
  * w_down (out, hidden), y (rows, out); act: GD_ACT_*.  Leading dimensions in elements (w_gate and w_up share one).  unaligned == 0 says that every
- * tensor of the calls starts at a multiple of 16 bytes and that the rows of dy are `out` or a multiple of 16 bytes apart (checked); != 0 takes any tensor, and
+ * tensor of the calls starts at a multiple of 16 bytes and that the rows of dy are `out` or a multiple of 16 bytes (up to 4 MiB) apart (checked); != 0 takes any tensor, and
  * sizes the workspace for that. */
 typedef struct gd_ffn_desc {
     int dtype, act;
