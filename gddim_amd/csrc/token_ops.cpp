@@ -84,27 +84,24 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
 long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
-    // Few rows: the weight-streaming kernel, up to 64, and further while 16 rows of x at a time do not read more of the weights than a launch costs
-    // (skinny_kernel has the figures; 128 x 256 x 688 takes 8.2 us instead of 19.6, 96 x 1024 x 4096 would take 41 instead of 33)
+    // Few rows: the weight-streaming kernel, where it is estimated to be faster than tiles.  Its time is what its workgroups read, mostly from L2: their rows of
+    // the weights and their rows of x, once for each workgroup (us of 64 x 1024 x 4096 in fp16 22.3, tiles 30.9; 96 rows 29.6, 32.8; 128 x 256 x 688 bf16 8.5, 18.8;
+    // 1 x 4096 x 14336 70, 85; but 16 x 4096 x 14336 97, 80; 64 rows 217, 91; 96 x 2048 x 8192 78, 46; 96 x 1024 x 4096 float32 61, 55)
+    double skinny_us = 1e30;
+    int skinny_m = 0, skinny_rows = 16, skinny_tiles = 0;
+    long long skinny_grid = 0;
     if ((kind == GEMM_GATE_UP || kind == GEMM_DOWN) && l.direct && l.q[0].M >= 1 && l.q[0].M <= 256) {
-        GemmProblem &q = l.q[0];
+        const GemmProblem &q = l.q[0];
         const int m_tiles = (q.M + 15) / 16;
-        if (q.M <= 64 || (double)m_tiles * (gated ? 2 : 1) * q.N * q.K * elem_size(dtype) <= (12 << 20)) {
-            l.tile = TILE_SKINNY;
-            q.splits = 1;
-            const long long slices = (q.N + 15) / 16;
-            int groups = (m_tiles + 2) / 3;
-            while (groups < m_tiles && slices * groups < cus) ++groups;
-            l.skinny_m = (m_tiles + groups - 1) / groups;
-            q.tiles_m = (m_tiles + l.skinny_m - 1) / l.skinny_m;
-            l.skinny_rows = 16;
-            while (l.skinny_m == 1 && l.skinny_rows > 4 && 2LL * m_tiles * ((q.N + l.skinny_rows - 1) / l.skinny_rows) <= cus) l.skinny_rows /= 2;
-            const long long grid = (q.N + 8LL * l.skinny_rows - 1) / (8LL * l.skinny_rows) * 8 * q.tiles_m;
-            if (grid > (1LL << 30)) return -1;
-            l.grid = l.blocks = (int)grid;
-            l.join_blocks = 0;
-            return 0;
-        }
+        const long long slices = (q.N + 15) / 16;
+        int groups = (m_tiles + 2) / 3;
+        while (groups < m_tiles && slices * groups < cus) ++groups;
+        skinny_m = (m_tiles + groups - 1) / groups;
+        skinny_tiles = (m_tiles + skinny_m - 1) / skinny_m;
+        while (skinny_m == 1 && skinny_rows > 4 && 2LL * m_tiles * ((q.N + skinny_rows - 1) / skinny_rows) <= cus) skinny_rows /= 2;
+        skinny_grid = (q.N + 8LL * skinny_rows - 1) / (8LL * skinny_rows) * 8 * skinny_tiles;
+        const int rows_read = skinny_rows * (gated ? 2 : 1) + (16 * skinny_m < q.M ? 16 * skinny_m : q.M);
+        if (skinny_grid <= (1LL << 30)) skinny_us = 3 + (dtype == GD_F32 ? 0.2e-6 : 0.14e-6) * (double)skinny_grid * q.K * (double)elem_size(dtype) * rows_read;
     }
     const int kstage = 128 / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
     struct Shape { GemmTile tile; int m, n; };
@@ -137,7 +134,10 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
             n += ((l.q[i].M + t.m - 1LL) / t.m) * tiles_n(l.q[i], t.n);
             out += (double)l.q[i].M * l.q[i].N * (gated ? 2 : 1);
         }
-        if (n > (1LL << 30)) return -1;
+        if (n > (1LL << 30)) {
+            if (skinny_us < 1e30) continue;
+            return -1;
+        }
         for (long long s = 1; s <= 16 && s <= stages && (s == 1 || stages / s >= 4); ++s) {
             const double per = (double)((stages + s - 1) / s), c = (double)((n * s + cus - 1) / cus);
             double us;
@@ -156,6 +156,16 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
                 chosen = t;
             }
         }
+    }
+    if (skinny_us <= best && skinny_us < 1e30) {
+        l.tile = TILE_SKINNY;
+        l.skinny_m = skinny_m;
+        l.skinny_rows = skinny_rows;
+        l.q[0].tiles_m = skinny_tiles;
+        l.q[0].splits = 1;
+        l.grid = l.blocks = (int)skinny_grid;
+        l.join_blocks = 0;
+        return 0;
     }
     l.tile = chosen.tile;
     const long long room = l.tile == TILE_256 ? cus : 2 * cus;
