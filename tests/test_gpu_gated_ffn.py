@@ -107,7 +107,7 @@ def test_more_tiles_than_workgroups(dev, size, typ):
 
 @pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("size", [(1, 8, 8, 8), (1, 520, 4104, 1032), (4, 1024, 40, 8), (16, 264, 4104, 2056), (17, 64, 2064, 1032), (48, 72, 136, 24), (64, 1000, 1024, 4104),
-                                  (100, 64, 136, 72), (256, 64, 200, 64), (255, 128, 352, 128)], ids=str)
+                                  (100, 64, 136, 72), (256, 64, 200, 64), (255, 128, 352, 128), (16, 2048, 8200, 2048), (40, 1032, 6152, 1032), (90, 1024, 4096, 1024)], ids=str)
 def test_few_rows(dev, size, typ):
     from gddim_amd import ops
     x, wg, wu, wd, _ = _inputs(dev, *size, TYPES[typ], 4)
