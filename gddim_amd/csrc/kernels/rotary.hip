@@ -16,13 +16,16 @@
 // Layout: a lane holds W pairs = two vectors of W channels.  (i, i + R/2) pairs: vector 0 from the first half, vector 1 from the second;
 // (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head: the weight-gradient sums stay in
 // registers (norm weights come from LDS, queries and keys apart).  lp lanes hold a head (with the norm a power of two: its sums are log2 lp permutes), 64 / lp
-// heads are in flight per wave.  Channels that pass through are pairs with phi = 0.
+// heads are in flight per wave.  Channels that pass through lie in lanes as pairs do, and every pair behind the last section is kept from the rotation by a
+// choice: a product with cos 0 = 1 and sin 0 = 0 would hand a neighbour's infinity on as NaN.
 //
 // W is 16 bytes of a type where pairs, strides and addresses allow it (the gradient in 16-bit types: 8), 8 bytes else, one pair where nothing is aligned.
 //
 // Measured, against the bytes at the 5.1 TB/s of a large copy: rotation of 46800 x 16 x 128 bf16 (383 MB) 80 us, 4.8 TB/s; norm and rotation of 65536 tokens x
 // (4 + 4) x 64 float32 (268 MB) 56 us, 4.8 TB/s; of 16382 x (16 + 4) x 128 bf16 (168 MB) 42 us, 4.0 TB/s, and its gradient (252 MB) 74 us, 3.4 TB/s, + 5 us for
 // the weights' sums.
+#include <type_traits>
+
 #include "../common.h"
 #include "../token_ops.h"
 
@@ -222,14 +225,22 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
     auto work = [&](int b, int n, int r, bool row_on) __attribute__((always_inline)) {
         const int seg = r >= p.heads[0];
         // index of a pair's two channels among the lane's 2W
-        auto turn = [&](float *y, int c) __attribute__((always_inline)) {
+        auto turn_pairs = [&](float *y, int c, auto all) __attribute__((always_inline)) {
+            constexpr bool whole = decltype(all)::value;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const int ia = HALVES ? i : 2 * i, ib = HALVES ? W + i : 2 * i + 1;
                 const float u = y[ia], v = y[ib];
-                y[ia] = u * cs[c][i] - v * sn[c][i];
-                y[ib] = u * sn[c][i] + v * cs[c][i];
+                const bool turns = whole || ch[c] * W + i < R2;
+                y[ia] = turns ? u * cs[c][i] - v * sn[c][i] : u;
+                y[ib] = turns ? u * sn[c][i] + v * cs[c][i] : v;
             }
+        };
+        // Norms in 16-bit types take heads that turn whole apart, by one branch of the wave: with the choice in them too, the gradient of 16 + 4 heads of 128
+        // channels took 82 us instead of 79.  The plain rotation (87 us with the branch, 82 without) and float32 (131 registers, 121) choose pair by pair.
+        auto turn = [&](float *y, int c) __attribute__((always_inline)) {
+            if (NORM && sizeof(T) == 2 && p.R == p.D) turn_pairs(y, c, std::true_type{});
+            else turn_pairs(y, c, std::false_type{});
         };
         if constexpr (NORM) {
             float ss = 0.f;

@@ -329,3 +329,74 @@ def test_axes_are_ready_for_any_stream(dev):
         got = ops.rotary(x, pos, axes)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+PARTIAL = [
+    # D, sections, head stride: vectors of 16 and 8 bytes and single pairs; lanes whose pairs turn in part, heads over more than 64 lanes
+    (64, (16, 16), 64), (64, (20, 16), 64), (72, (24, 24), 80), (40, (8, 4), 44), (24, (8, 2), 25), (33, (4, 6), 33), (260, (100, 60), 260), (512, (128, 66), 513), (16, (2,), 16),
+]
+
+
+def _strided(t, apart, dev):
+    """t (B, N, heads, D) on the device with heads `apart` elements from each other"""
+    big = torch.zeros(t.shape[:3] + (apart,), dtype=t.dtype, device=dev)
+    big[..., :t.shape[3]] = t.to(dev)
+    return big[..., :t.shape[3]]
+
+
+@pytest.mark.parametrize("paired", ["interleaved", "halves"])
+@pytest.mark.parametrize("typ", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("form", PARTIAL, ids=str)
+def test_channels_behind_the_sections_pass_through(dev, form, typ, paired):
+    """as they are, whatever lies beside them: infinities, NaN and the sign of zeros"""
+    from gddim_amd import ops
+    D, sections, apart = form
+    R, dtype = sum(sections), TYPES[typ]
+    g = _gen(31)
+    x = torch.randn(2, 5, 3, D, generator=g).to(dtype)
+    special = torch.tensor([float("inf"), float("-inf"), float("nan"), -0.0, 0.0])
+    rest = x[..., R:]
+    at = torch.rand(rest.shape, generator=g) < 0.4
+    rest[at] = special[torch.randint(0, 5, (int(at.sum()),), generator=g)].to(dtype)
+    pos = torch.randint(-40, 40, (5, len(sections)), generator=g)
+    phi = ref.angles(pos, sections, 10000.0, 2, 5)
+    axes = ops.RotaryAxes(sections, paired=paired, device=dev)
+    for inverse in (False, True):
+        got = ops.rotary(_strided(x, apart, dev), pos.to(dev), axes, inverse=inverse).cpu()
+        want, mag = ref.rotate(x.double(), phi, sections, paired, inverse)
+        ref.assert_within(got[..., :R], want[..., :R], ref.bound(want, mag, ref.ROTATION, dtype)[..., :R])
+        out, nan = got[..., R:], torch.isnan(rest)
+        assert torch.equal(torch.isnan(out), nan)
+        assert torch.equal(out[~nan], rest[~nan]) and torch.equal(torch.signbit(out[~nan]), torch.signbit(rest[~nan]))
+
+
+@pytest.mark.parametrize("paired", ["interleaved", "halves"])
+@pytest.mark.parametrize("typ", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("form", PARTIAL, ids=str)
+def test_gradients_behind_the_sections_stay_their_own(dev, form, typ, paired):
+    """an infinite gradient of a channel that passes through is its weight's alone; an infinite input leaves zeros of its head's other channels"""
+    from gddim_amd import ops
+    D, sections, apart = form
+    R, dtype, eps = sum(sections), TYPES[typ], 1e-5
+    g = _gen(32)
+    q, gy = (torch.randn(1, 4, 2, D, generator=g).to(dtype) for _ in range(2))
+    q[0, 1, 0, R] = q[0, 1, 0, R].abs() + 0.5  # (a product of an infinity with zero would be NaN by the formula)
+    w, pos = (1 + 0.3 * torch.randn(D, generator=g)).to(dtype), torch.randint(-40, 40, (4, len(sections)), generator=g)
+    phi = ref.angles(pos, sections, 10000.0, 1, 4)
+    axes = ops.RotaryAxes(sections, paired=paired, device=dev)
+    gy[0, 1, 0, R] = float("inf")
+    qd, gd = _strided(q, apart, dev), _strided(gy, apart, dev)
+    dq, dk, dwq, dwk = ops.qk_norm_rotary_backward(gd, gd, qd, qd, w.to(dev), w.to(dev), pos.to(dev), axes, eps=eps)
+    want, mag, dww, dwm, n = ref.norm_rotary_backward(gy.double(), q.double(), w.double(), phi, sections, paired, eps)
+    others = torch.arange(D) != R
+    limit = ref.bound(dww, dwm, n + 128, dtype)
+    for dw in (dwq, dwk):
+        assert dw[R] == float("inf")
+        ref.assert_within(dw[others.to(dev)], dww[others], limit[others], "dw")
+    heads = torch.ones(1, 4, 2, dtype=torch.bool)
+    heads[0, 1, 0] = False
+    ref.assert_within(dq.cpu()[heads], want[heads], ref.bound(want, mag, n, dtype)[heads], "dx")
+
+    q[0, 2, 1, R] = float("inf")
+    out = ops.qk_norm_rotary(_strided(q, apart, dev), qd, w.to(dev), w.to(dev), pos.to(dev), axes, eps=eps)[0].cpu()
+    assert torch.isnan(out[0, 2, 1, R]) and (out[0, 2, 1][others] == 0).all()
