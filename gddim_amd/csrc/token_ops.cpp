@@ -69,7 +69,9 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
     q.N = (int)(bkc ? b[0].rows : b[0].cols);
     q.K = (int)(akc ? a[0].cols : a[0].rows);
     q.parts = parts;
-    auto bytes = [&](const Matrix &m) { return m.rows ? ((m.rows - 1) * m.ld + m.cols) * (long long)es : 0; };
+    // Whole dwords: a read is held against the end dword by dword, and of a 16-bit matrix with an odd number of columns the last element lies in the first half of
+    // one (the other half is padding of the row, or memory of the same aligned dword; it only meets columns that are not stored)
+    auto bytes = [&](const Matrix &m) { return m.rows ? (((m.rows - 1) * m.ld + m.cols) * (long long)es + 3) / 4 * 4 : 0; };
     q.lda = a[0].ld * es; q.ldb = b[0].ld * es;
     q.a_bytes = bytes(a[0]); q.b_bytes = bytes(b[0]);
     for (int s = 0; s < 2; ++s) {

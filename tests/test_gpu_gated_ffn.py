@@ -355,3 +355,28 @@ def test_refusals_on_the_gpu(dev):
         with pytest.raises(GddimError):
             call()
             pytest.fail("call %d was not refused" % i)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("columns", [49, 50, 51, 129, 130, 255])
+@pytest.mark.parametrize("which", ["x", "w_gate and w_up", "w_down"])
+def test_odd_columns_of_padded_rows(dev, which, columns, typ):
+    """matrices whose rows are whole 16-byte pieces apart and hold no whole number of them: their last row's last element ends the memory that a product
+    reads, and counts for much here"""
+    M, D, F, O, dtype = 70, 72, 80, 40, TYPES[typ]
+    if which == "w_down":
+        F = columns
+    else:
+        D = columns
+    x, wg, wu, wd, dy = _inputs(dev, M, D, F, O, dtype, 21)
+    for t in (x, wg, wu, wd):
+        t[-1, -1] = 12.0
+    wide = lambda t: torch.cat((t, torch.full((t.shape[0], -t.shape[1] % 8 + 8), float("nan"), dtype=dtype, device=dev)), 1)[:, :t.shape[1]]
+    args = [wide(x) if which == "x" else x] + [wide(t) if which == "w_gate and w_up" else t for t in (wg, wu)] + [wide(wd) if which == "w_down" else wd]
+    want = ref.gated_ffn(x, wg, wu, wd, "silu", dtype, dy)
+    for g, w, what in zip(_run(*args, dy, "silu"), want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        if dtype == torch.float16:  # 12^5 = 248832 is past its range: values of 65520 and more round to infinity
+            over = w.val.abs() - w.err >= 65520
+            assert (g[over].double() == w.val[over].sign() * float("inf")).all()
+            g, w = g.masked_fill(over, 0), ref.V(w.val.masked_fill(over, 0), w.err)
+        _check(g, w, what)
