@@ -82,6 +82,8 @@ GemmProblem problem(const Matrix *a, bool akc, const Matrix *b, bool bkc, int pa
     return q;
 }
 
+constexpr long long MAX_THREADS = (1LL << 32) - 1;  // of a launch: more are refused
+
 // tile and split of a launch; returns the floats of partial sums it needs, or -1 (more workgroups than a grid holds)
 long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
@@ -103,7 +105,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
         while (skinny_m == 1 && skinny_rows > 4 && 2LL * m_tiles * ((q.N + skinny_rows - 1) / skinny_rows) <= cus) skinny_rows /= 2;
         skinny_grid = (q.N + 8LL * skinny_rows - 1) / (8LL * skinny_rows) * 8 * skinny_tiles;
         const int rows_read = skinny_rows * (gated ? 2 : 1) + (16 * skinny_m < q.M ? 16 * skinny_m : q.M);
-        if (skinny_grid <= (1LL << 30)) skinny_us = 3 + (dtype == GD_F32 ? 0.2e-6 : 0.14e-6) * (double)skinny_grid * q.K * (double)elem_size(dtype) * rows_read;
+        if (skinny_grid * 1024 <= MAX_THREADS) skinny_us = 3 + (dtype == GD_F32 ? 0.2e-6 : 0.14e-6) * (double)skinny_grid * q.K * (double)elem_size(dtype) * rows_read;
     }
     const int kstage = 128 / (int)elem_size(dtype);  // gated_ffn_gemm.h: bytes of k a stage
     struct Shape { GemmTile tile; int m, n; };
@@ -130,9 +132,10 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     Shape chosen = shapes[0];
     for (const Shape &t : shapes) {
         if (t.tile == TILE_256 && (dtype == GD_F32 || !l.direct)) continue;
-        long long n = 0;
+        long long n = 0, joins = 0;
         double out = 0;
         for (int i = 0; i < l.problems; ++i) {
+            joins += (l.q[i].M * ((l.q[i].N + 3LL) / 4) + 255) / 256 * 256;
             n += ((l.q[i].M + t.m - 1LL) / t.m) * tiles_n(l.q[i], t.n);
             out += (double)l.q[i].M * l.q[i].N * (gated ? 2 : 1);
         }
@@ -141,6 +144,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
             return -1;
         }
         for (long long s = 1; s <= 16 && s <= stages && (s == 1 || stages / s >= 4); ++s) {
+            if (s > 1 && joins > MAX_THREADS) break;
             const double per = (double)((stages + s - 1) / s), c = (double)((n * s + cus - 1) / cus);
             double us;
             if (t.tile == TILE_256) us = c * ((kind != GEMM_DW ? 1.9 : n * s < cus ? 1.7 : 2.1) * per + 3) + 5;
@@ -188,7 +192,7 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
         }
         join += q.join_threads;
     }
-    if (blocks > (1LL << 30) || join / 256 > (1LL << 30)) return -1;
+    if (blocks > (1LL << 30)) return -1;
     l.join_blocks = (int)(join / 256);
     l.blocks = (int)blocks;
     l.grid = (int)(blocks < room ? blocks : room / 8 * 8);  // a workgroup's pieces stay on its XCD

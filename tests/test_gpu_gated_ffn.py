@@ -380,3 +380,21 @@ def test_odd_columns_of_padded_rows(dev, which, columns, typ):
             assert (g[over].double() == w.val[over].sign() * float("inf")).all()
             g, w = g.masked_fill(over, 0), ref.V(w.val.masked_fill(over, 0), w.err)
         _check(g, w, what)
+
+
+def test_few_rows_against_very_many(dev):
+    """2^26 rows of the weights: as workgroups of 16 rows each they would be 2^32 threads, more than a launch holds"""
+    from gddim_amd import ops
+    M, D, F, O, dtype = 2, 8, 1 << 26, 8, torch.bfloat16
+    x, wg, wu, _, _ = _inputs(dev, M, D, F, 1, dtype, 22)
+    at = torch.tensor([0, 1, 15, 16, 12345678, F // 2, F - 17, F - 2, F - 1], device=dev)
+    wd = torch.zeros(O, F, dtype=dtype, device=dev)
+    wd[:, at] = torch.randn(O, len(at), generator=torch.Generator(dev).manual_seed(23), device=dev).to(dtype)
+    y, saved = ops.gated_ffn(x, wg, wu, wd, save=True)
+    gate, up = ref.product(ref.V(x.double()), ref.V(wg.double())), ref.product(ref.V(x.double()), ref.V(wu.double()))
+    _check(saved[0], gate, "gate")
+    _check(saved[1], up, "up")
+    hidden = (ref.act(gate, "silu")[0] * up).rounded(dtype)
+    _check(saved[2], hidden, "hidden")
+    # all other products are zeros, which round nothing
+    _check(y, ref.product(ref.V(hidden.val[:, at], hidden.err[:, at]), ref.V(wd[:, at].double())).rounded(dtype), "y")

@@ -182,3 +182,49 @@ def test_rotary_axes_copies(native_lib):
     assert other.frequencies.data_ptr() != axes.frequencies.data_ptr() and other.sections == axes.sections
     with pytest.raises(AttributeError):  # a kernel reads as many of them as the sections say
         axes.frequencies = torch.ones(1)
+
+
+@pytest.fixture(scope="module")
+def launches(tmp_path_factory):
+    """The entry points' host code over launchers that only write down what they are asked for (tests/token_launches.cpp)."""
+    import os
+    import subprocess
+    from gddim_amd import build
+    here = os.path.dirname(os.path.abspath(__file__))
+    lib = str(tmp_path_factory.mktemp("launches") / "token_launches.so")
+    subprocess.check_call([build._hipcc(), "-x", "hip", "--cuda-host-only", "-O1", "-std=c++17", "-fPIC", "-shared", os.path.join(here, "token_launches.cpp"), "-o", lib])
+    lib = ctypes.CDLL(lib)
+    lib.gd_gated_ffn_workspace.restype = ctypes.c_longlong
+    ll, p = ctypes.c_longlong, ctypes.c_void_p
+    lib.gd_gated_ffn.argtypes, lib.gd_gated_ffn_backward.argtypes = [p] * 11, [p, p, ll] + [p] * 13
+
+    def ask(d, out):
+        lib.forget_launches()
+        at = 1 << 20  # an address that nothing reads
+        assert lib.gd_gated_ffn(d, at, at, at, at, None, None, at, at, at, None) == 0
+        assert lib.gd_gated_ffn_backward(d, at, out, at, at, at, at, at, at, at, at, at, at, at, at, None) == 0
+        rows = []
+        for i in range(lib.launches()):
+            row = (ctypes.c_longlong * 6)()
+            lib.launch(i, row)
+            rows.append(list(row))
+        assert [r[0] for r in rows] == [0, 1, 2, 3, 4]
+        return rows, [at + lib.gd_gated_ffn_workspace(d, b) for b in (0, 1)]
+
+    return ask
+
+
+def test_c_gated_ffn_launches_are_within_a_grid_s_limits(launches):
+    """no launch of 2^32 threads or more, and none whose partial sums leave the workspace"""
+    for dtype in (0, 1, 2):
+        for rows in (1, 2, 16, 17, 33, 100, 256, 1000, 70001):
+            for in_, hidden, out in ((8, 8, 8), (1024, 4096, 1024), (8, 1 << 22, 8), (8, 1 << 26, 8), (16, (1 << 28) + 16, 8), (8, 64, 1 << 26), (8, 1 << 30, 8), (64, 72, 1 << 30)):
+                for unaligned in (0, 1):
+                    if rows * hidden >= 1 << 38 or rows * out >= 1 << 38:  # (half a terabyte: no card holds it)
+                        continue
+                    d = _ffn(dtype=dtype, rows=rows, in_=in_, hidden=hidden, out=out, unaligned=unaligned, ld_x=in_, ld_w_in=in_, ld_w_down=hidden)
+                    shapes, ends = launches(d, out)
+                    for kind, tile, grid, threads, join, partial in shapes:
+                        what = (dtype, rows, in_, hidden, out, unaligned, kind, tile)
+                        assert 0 < grid * threads < 1 << 32 and 0 <= join * 256 < 1 << 32, what
+                        assert partial <= ends[kind > 1], what
