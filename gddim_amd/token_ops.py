@@ -319,7 +319,8 @@ def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
 
 def gated_ffn_backward(dy, x, w_gate, w_up, w_down, saved, act="silu"):
     """Gradients (dx, dw_gate, dw_up, dw_down) of gated_ffn from that of its result and what the call with save=True kept (left as it was).  The
-    same bits every time."""
+    same bits every time.  The gradients of both projections are rounded to x's type before they are summed: in float16 past 65504 infinite, under
+    2^-25 zero."""
     x_in = x
     x, w_gate, w_up, w_down, fields = _check_ffn(x, w_gate, w_up, w_down, act)
     M, D, F, O = fields[2:6]

@@ -409,7 +409,9 @@ long long gd_gated_ffn_workspace(const gd_ffn_desc *d, int backward);
 int gd_gated_ffn(const gd_ffn_desc *d, const void *x, const void *w_gate, const void *w_up, const void *w_down, float *gate_dev, float *up_dev,
                  void *hidden_dev, void *y, void *workspace_dev, void *stream);
 /* Gradients from dy (rows, out; rows ld_dy apart) and what the forward call kept: dx (rows, in), dw_gate, dw_up (hidden, in), dw_down (out, hidden), all
- * dense.  workspace_dev: gd_gated_ffn_workspace(d, 1) bytes, 16-byte aligned.  The same bits every time. */
+ * dense.  workspace_dev: gd_gated_ffn_workspace(d, 1) bytes, 16-byte aligned.  The same bits every time.  The gradients of the two projections, dh (.) up (.)
+ * act'(gate) and dh (.) act(gate) with dh = dy w_down, are rounded to the tensors' type before they are summed to dx, dw_gate and dw_up: in fp16 what is past
+ * 65504 becomes infinite and what is under 2^-25 zero, also where the sums would lie in its range. */
 int gd_gated_ffn_backward(const gd_ffn_desc *d, const void *dy, long long ld_dy, const void *x, const void *w_gate, const void *w_up,
                           const void *w_down, const float *gate, const float *up, const void *hidden, void *dx, void *dw_gate, void *dw_up,
                           void *dw_down, void *workspace_dev, void *stream);

@@ -398,3 +398,26 @@ def test_few_rows_against_very_many(dev):
     _check(saved[2], hidden, "hidden")
     # all other products are zeros, which round nothing
     _check(y, ref.product(ref.V(hidden.val[:, at], hidden.err[:, at]), ref.V(wd[:, at].double())).rounded(dtype), "y")
+
+
+@pytest.mark.parametrize("size", [(70, 64, 72, 40), (3, 64, 72, 40), (33, 65, 71, 39), (300, 256, 688, 256)], ids=str)
+@pytest.mark.parametrize("scale", [-18, -14, -8, 9])
+def test_gradients_of_small_and_large_scale_in_fp16(dev, scale, size):
+    """dgate and dup are rounded to fp16 before they are summed: down to its subnormal step, 2^-24, and within 65504 as long as they stay so themselves"""
+    x, wg, wu, wd, dy = _inputs(dev, *size, torch.float16, 24)
+    dy = dy * 2.0 ** scale
+    want = ref.gated_ffn(x, wg, wu, wd, "silu", torch.float16, dy)
+    for g, w, what in zip(_run(x, wg, wu, wd, dy, "silu"), want, ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        _check(g, w, what)
+
+
+def test_hidden_gradients_past_the_range_of_fp16(dev):
+    """dgate = 65536 is an infinity before it is summed; bf16 and float32 hold it"""
+    for typ, dtype in TYPES.items():
+        x, w, dy = (torch.full((1, 1), v, dtype=dtype, device=dev) for v in (32.0, 1.0, 2048.0))
+        dx, dwg, _, dwd = _run(x, w, w, w, dy, "silu")[1:]
+        assert dwd.item() == (float("inf") if typ == "f16" else 2048.0 * 1024.0)  # the result itself
+        if typ == "f16":
+            assert dwg.item() == float("inf") and dx.item() == float("inf")
+        else:
+            assert dwg.item() == 65536.0 * 32.0 and dx.item() == 65536.0 * 2
