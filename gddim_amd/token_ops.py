@@ -49,6 +49,9 @@ def _on_gpu(t, name):
     torch = _torch()[0]
     if not isinstance(t, torch.Tensor):
         raise GddimError("%s: expected a torch tensor, got %s" % (name, type(t).__name__))
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and forward.unpack_dual(t).tangent is not None:  # (no level, no tangents: asked first, in a quarter of the time)
+        raise GddimError("%s carries a forward-mode tangent: the token operators have no forward-mode derivative" % name)
     if not t.is_cuda:
         raise GddimError("gddim_amd operators run on the GPU only (%s is a %s tensor); there is no CPU fallback" % (name, t.device))
     if t.requires_grad and torch.is_grad_enabled():

@@ -107,3 +107,21 @@ def test_gradients_through_norms_and_feed_forward(native_lib):
     for i, (a, b) in enumerate(zip(got, want)):
         # float32 sums of up to 344 terms, three in a row: 3 * 344 * 2^-24 = 6e-5, and the norms' 64
         assert float((a.cpu().double() - b).abs().max()) < 1e-4 * float(b.abs().max()), i
+
+
+def test_forward_mode_tangents_are_refused(native_lib):
+    from torch.autograd import forward_ad
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    dev = torch.device("cuda", 0)
+    x, w, pos = torch.randn(1, 2, 1, 4, device=dev), torch.randn(4, device=dev), torch.zeros(2, 1, device=dev)
+    axes, m, a = ops.RotaryAxes((4,), device=dev), torch.randn(2, 4, device=dev), torch.randn(4, 4, device=dev)
+    y, saved = ops.gated_ffn(m, a, a, a, save=True)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rotary(x, dual(pos), axes), lambda: ops.qk_norm_rotary(x, dual(x), w, w, pos, axes), lambda: ops.qk_norm_rotary(x, x, dual(w), w, pos, axes),
+                     lambda: ops.qk_norm_rotary_backward(x, dual(x), x, x, w, w, pos, axes), lambda: ops.gated_ffn(m, a, dual(a), a), lambda: ops.gated_ffn(m, a, a, dual(a)),
+                     lambda: ops.gated_ffn_backward(dual(m), m, a, a, a, saved), lambda: ops.gated_ffn_backward(m, m, a, a, a, (dual(saved[0]),) + saved[1:])):
+            with pytest.raises(GddimError, match="tangent"):
+                call()
+        assert torch.equal(ops.gated_ffn(m, a, a, a), y)  # tensors without one are taken inside a level, too

@@ -228,3 +228,21 @@ def test_c_gated_ffn_launches_are_within_a_grid_s_limits(launches):
                         what = (dtype, rows, in_, hidden, out, unaligned, kind, tile)
                         assert 0 < grid * threads < 1 << 32 and 0 <= join * 256 < 1 << 32, what
                         assert partial <= ends[kind > 1], what
+
+
+def test_forward_mode_tangents_are_refused(native_lib):
+    """a dual tensor does not require grad; its tangent would be lost without a word"""
+    from torch.autograd import forward_ad
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    axes, x, w, pos = ops.RotaryAxes((4,), device="cpu"), torch.zeros(1, 2, 1, 4), torch.zeros(4), torch.zeros(2, 1)
+    m, a, b = torch.zeros(2, 4), torch.zeros(6, 4), torch.zeros(4, 6)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rotary(dual(x), pos, axes), lambda: ops.qk_norm_rotary(dual(x), x, w, w, pos, axes),
+                     lambda: ops.qk_norm_rotary_backward(x, x, dual(x), x, w, w, pos, axes), lambda: ops.gated_ffn(dual(m), a, a, b),
+                     lambda: ops.gated_ffn_backward(m, dual(m), a, a, b, (m, m, m))):
+            with pytest.raises(GddimError, match="tangent"):
+                call()
+        with pytest.raises(GddimError, match="GPU only"):
+            ops.rotary(x, pos, axes)
