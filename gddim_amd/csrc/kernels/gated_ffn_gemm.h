@@ -70,7 +70,8 @@ template <int ACT> __device__ __forceinline__ void act_grad(float z, float &a, f
     } else {
         const float t = fast_tanh(0.79788456080286536f * (z + 0.044715f * z * z * z));
         a = 0.5f * z * (1.f + t);
-        da = 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
+        const float z2 = fminf(z * z, 1e30f);  // past |z| = 10 the term is 0, and stays 0 where the square overflows
+        da = 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z2);
     }
 }
 

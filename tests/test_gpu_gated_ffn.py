@@ -421,3 +421,18 @@ def test_hidden_gradients_past_the_range_of_fp16(dev):
             assert dwg.item() == float("inf") and dx.item() == float("inf")
         else:
             assert dwg.item() == 65536.0 * 32.0 and dx.item() == 65536.0 * 2
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("exponent", [10, 40, 62, 65, 90, 120])
+def test_activations_of_very_large_projections(dev, exponent, typ, kind):
+    """z = +-2^n: the activation is z or 0, its derivative 1 or 0, also where z^2 and z^3 overflow; powers of two, so nothing rounds"""
+    dtype = TYPES[typ]
+    for sign in (1.0, -1.0):
+        z, small, one = sign * 2.0 ** exponent, 2.0 ** -100, torch.ones(1, 1, dtype=dtype, device=dev)
+        x, wu = one * z, one * small
+        y, dx, dwg, _, dwd = _run(x, one, wu, one, one, kind)  # gate = z, up = z 2^-100
+        want = (z * z * small, 2 * z * small, z * small * z, z * z * small) if sign > 0 else (0.0,) * 4
+        for g, w, what in zip((y, dx, dwg, dwd), want, ("y", "dx", "dw_gate", "dw_down")):
+            assert g.item() == (w if abs(w) < 2.0 ** 128 else float("inf")), (what, g.item(), w)  # (past the range of both types)
