@@ -147,6 +147,8 @@ def _rotary_desc(x, pos, axes):
     B, N, _, D = x.shape
     _on_gpu(pos, "pos")
     kind = pos_types.get(pos.dtype)
+    if kind == 2 and pos.is_neg():
+        raise GddimError("pos is a lazily negated view (of a conjugate): its memory holds the other sign; give pos.resolve_neg()")
     if kind is None:
         raise GddimError("pos is %s; int32, int64 and float32 positions are supported" % pos.dtype)
     index = x.get_device()
@@ -247,6 +249,8 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 def _rows(t, columns):
     """t (..., columns) as a matrix with adjacent columns and rows at least a row apart: a view where there is one"""
+    if columns == 1:
+        t = t.resolve_neg()  # (a lazily negated view has strides of two or more, the imaginary part of a conjugate; with more columns it is copied below)
     if t.dim() == 2 and t.is_contiguous():
         return t
     if t.dim() != 2:

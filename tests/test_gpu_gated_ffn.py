@@ -436,3 +436,14 @@ def test_activations_of_very_large_projections(dev, exponent, typ, kind):
         want = (z * z * small, 2 * z * small, z * small * z, z * z * small) if sign > 0 else (0.0,) * 4
         for g, w, what in zip((y, dx, dwg, dwd), want, ("y", "dx", "dw_gate", "dw_down")):
             assert g.item() == (w if abs(w) < 2.0 ** 128 else float("inf")), (what, g.item(), w)  # (past the range of both types)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 4])
+def test_lazily_negated_tensors(dev, which):
+    """matrices of one column are taken with any stride, the imaginary part of a conjugate among them"""
+    args = list(_inputs(dev, 5, 1, 1, 1, torch.float32, 25))
+    want = _run(*[-t if i == which else t for i, t in enumerate(args)], "gelu")
+    args[which] = torch.complex(args[which], args[which]).conj().imag
+    assert args[which].is_neg()
+    for g, w in zip(_run(*args, "gelu"), want):
+        assert torch.equal(g, w)

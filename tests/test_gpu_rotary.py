@@ -400,3 +400,19 @@ def test_gradients_behind_the_sections_stay_their_own(dev, form, typ, paired):
     q[0, 2, 1, R] = float("inf")
     out = ops.qk_norm_rotary(_strided(q, apart, dev), qd, w.to(dev), w.to(dev), pos.to(dev), axes, eps=eps)[0].cpu()
     assert torch.isnan(out[0, 2, 1, R]) and (out[0, 2, 1][others] == 0).all()
+
+
+def test_lazily_negated_positions_are_refused(dev):
+    """the imaginary part of a conjugate is a view with a sign to come: its memory holds the other one"""
+    from gddim_amd import ops
+    from gddim_amd._abi import GddimError
+    x, axes = torch.randn(1, 5, 2, 16, generator=_gen(40)).to(dev), ops.RotaryAxes((8, 8), device=dev)
+    z = torch.complex(torch.zeros(5, 2), torch.randint(-9, 9, (5, 2), generator=_gen(41)).float()).to(dev)
+    pos = z.conj().imag
+    assert pos.is_neg()
+    for call in (lambda: ops.rotary(x, pos, axes), lambda: ops.qk_norm_rotary(x, x, None, None, pos, axes), lambda: ops.qk_norm_rotary_backward(x, x, x, x, None, None, pos, axes)):
+        with pytest.raises(GddimError, match="resolve_neg"):
+            call()
+    assert torch.equal(ops.rotary(x, pos.resolve_neg(), axes), ops.rotary(x, -z.imag.contiguous(), axes))
+    zx = torch.complex(x, x)
+    assert torch.equal(ops.rotary(zx.conj().imag, z.imag, axes), ops.rotary(-x, z.imag, axes))  # channels two apart: copied, and the sign with them
