@@ -1,4 +1,5 @@
 // C entry points of the token operators: argument checks, then the launchers of kernels/.
+#include <cfloat>
 #include <cstdint>
 
 #include "common.h"
@@ -347,7 +348,7 @@ int gd_qk_norm_rotary(const gd_rotary_desc *d, const gd_heads *q, const gd_heads
     RotaryParams p{};
     GD_TRY(fill_rotary(p, d, who));
     GD_CHECK(heads_q >= 1 && heads_k >= 1 && heads_q <= 65535 && heads_k <= 65535, "%s: %d / %d heads outside [1, 65535]", who, heads_q, heads_k);
-    GD_CHECK(eps >= 0.f, "%s: negative eps", who);
+    GD_CHECK(eps >= 0.f && eps <= FLT_MAX, "%s: eps %g is negative or not a finite float32", who, eps);
     const bool empty = (long long)p.batch * p.tokens == 0;
     GD_TRY(view(p.x[0], q, empty, who, "q"));
     GD_TRY(view(p.x[1], k, empty, who, "k"));
@@ -369,7 +370,7 @@ int gd_qk_norm_rotary_backward(const gd_rotary_desc *d, const gd_heads *dq_out, 
     RotaryParams p{};
     GD_TRY(fill_rotary(p, d, who));
     GD_CHECK(heads_q >= 1 && heads_k >= 1 && heads_q <= 65535 && heads_k <= 65535, "%s: %d / %d heads outside [1, 65535]", who, heads_q, heads_k);
-    GD_CHECK(eps >= 0.f, "%s: negative eps", who);
+    GD_CHECK(eps >= 0.f && eps <= FLT_MAX, "%s: eps %g is negative or not a finite float32", who, eps);
     GD_CHECK(workspace_dev, "%s: null workspace", who);
     const bool empty = (long long)p.batch * p.tokens == 0;
     GD_TRY(view(p.dy[0], dq_out, empty, who, "dq_out"));

@@ -384,7 +384,7 @@ typedef struct gd_rotary_desc {
 /* out = rotation(x); inverse != 0: the rotation back, which is also the gradient.  x and out may not overlap. */
 int gd_rotary(const gd_rotary_desc *d, const gd_heads *x, const gd_heads *out, int heads, int inverse, void *stream);
 /* out = rotation(w (.) x / sqrt(mean_D x^2 + eps)) for the queries and the keys of every token in one pass; w_q / w_k (D) of the tensors'
- * type, or fp32 with w_f32 != 0, or null (ones). */
+ * type, or fp32 with w_f32 != 0, or null (ones); eps: 0 to the largest float32. */
 int gd_qk_norm_rotary(const gd_rotary_desc *d, const gd_heads *q, const gd_heads *k, const gd_heads *q_out, const gd_heads *k_out, int heads_q,
                       int heads_k, const void *w_q, const void *w_k, int w_f32, float eps, void *stream);
 /* Its gradient: dq, dk of the inputs and dw_q, dw_k (types as w; null where the weight is) from the outputs' gradients.  workspace_dev holds

@@ -246,3 +246,14 @@ def test_forward_mode_tangents_are_refused(native_lib):
                 call()
         with pytest.raises(GddimError, match="GPU only"):
             ops.rotary(x, pos, axes)
+
+
+def test_c_entry_points_refuse_an_eps_past_float32(native_lib):
+    """1e39 reaches the C interface as an infinity, and every head would come out as zeros"""
+    from gddim_amd._abi import Heads
+    h, d = ctypes.byref(Heads(64, 64, 16, 16)), _desc()
+    for eps in (1e39, float("inf"), -1.0, float("nan")):
+        assert native_lib.gd_qk_norm_rotary(d, h, h, h, h, 1, 1, None, None, 0, eps, None) != 0
+        assert b"eps" in native_lib.gd_last_error()
+        assert native_lib.gd_qk_norm_rotary_backward(d, h, h, h, h, h, h, 1, 1, None, None, 0, eps, 64, None, None, None) != 0
+        assert b"eps" in native_lib.gd_last_error()
