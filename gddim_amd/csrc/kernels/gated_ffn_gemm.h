@@ -13,21 +13,22 @@
 // (lane % 32) and k = 8 (lane / 32) .. + 7 of a 32-row x 16-k block (16-bit types; the transposing LDS read gathers it where k is not adjacent), one
 // v_mfma_f32_32x32x16; in float32 four values, four v_mfma_f32_32x32x2.  A sum does not care which k a lane holds as long as both operands agree, so
 // both layouts and all types share one loop.  The MFMA's first operand is B: a lane then ends with groups of four ADJACENT n of one row m.
-// In LDS a KC row is one line of 128 bytes (with stages of 64 bytes the requests to L2 doubled and became the bound: y of 16384 x 1024 x 4096 in 153 us
-// instead of 129), 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k rows, pieces moved by k.  No bank conflicts either way (counted).
+// In LDS a KC row is one line of 128 bytes, what L2 is asked for at a time, 8 pieces of 16, piece c of row r at c ^ swizzle(r); other operands keep their k
+// rows, pieces moved by k.  No bank conflicts either way (counted: none, but for the gated epilogue's, 6 % of that kernel's LDS cycles).
 // Memory goes to LDS directly, 16 bytes a lane (buffer_load ... lds: no registers, out-of-range pieces arrive as zeros); where rows are not whole
 // 16-byte pieces, through registers.
 // Two stages lie in LDS.  A step multiplies fragments that were read during the step before, those of the next are read between its products: when a stage's
 // last step begins all of it has been read, and the stage after the next is requested into its place, a whole stage (2048 MFMA cycles a SIMD of a 256 x
 // 256 tile) before it is needed.
 //
-// What bounds them: with k long, the matrix core at the clock that the card's power leaves it (1.64 to 1.75 GHz in bf16: 16384 x 1024 x 4096, products of 137
-// to 412 GFLOP, at 0.95 to 1.17 PFLOP/s; a library product of these shapes reaches 0.91 to 1.38), in float32 its rate (133 to 138 TFLOP/s; library 138 to 150).
+// What bounds them: in float32 with k long the matrix core's rate (8192 x 1024 x 4096, products of 69 to 206 GFLOP, at 124 to 138 TFLOP/s; library products 126 to
+// 151).  In bf16 at 16384 x 1024 x 4096 the products of 137 to 412 GFLOP run at 0.97 to 1.17 PFLOP/s (library products of these shapes: 0.87 to 1.38), 0.78 where gate and
+// up are kept and 0.48 in dhidden, whose epilogues move 671 and 805 MB; the clock is 1.9 to 2.1 GHz then and the matrix core busy in 46 to 59 % of the cycles (37 and
+// 22 in these two): the rest is waiting, for a stage at its barrier or in the epilogue.
 //
 // All sums are float32 in the matrix core's accumulators.  Rounded to the tensors' type are only operands of a next product, as the 16-bit matrix core
-// wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients at
-// 1.8 times the error of one final rounding (relative 3.1e-3 instead of 2.4e-3; 1.7e-3 is the final rounding alone; a single row, where few terms dominate a
-// sum, up to 2.9e-3).
+// wants them -- h, dgate, dup -- and the results.  gate and up, which a training step keeps, stay float32: rounded to bf16 they put the gradients of dx, dWg and dWu
+// at a relative error of 2.9e-3 to 3.1e-3 (2048 x 1024 x 2736) instead of 2.4e-3, of which the final rounding alone is 1.7e-3.
 #pragma once
 #include "../common.h"
 #include "../token_ops.h"
@@ -309,8 +310,7 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // 32 rows of accumulators from LDS through the epilogue.  Inside the matrix (all of a large one) the loop is stripped of bounds, of 64-bit
-// address arithmetic and of the choice of activation.  Row by row through LDS, because accumulators that met the epilogue in place went to scratch
-// memory (dhidden of 16384 x 1024 x 4096 977 us instead of 284).
+// address arithmetic and of the choice of activation.  Row by row through LDS, because accumulators that met the epilogue in place went to scratch memory.
 template <typename T, int EPI, int ACT>
 __device__ __forceinline__ void rows_inside(const GemmProblem &q, const char *mine, int m, int n, int lane) {
     constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
@@ -606,9 +606,10 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void gemm_kernel(const GemmLaunch p
 // Few rows: the weights' bytes are the time, so nothing is staged.  A workgroup of 16 waves takes 16 MT rows of x and ROWS rows of the weights (of gate and of
 // up), a wave every 16th 128-byte line of them, straight from memory into the operand registers of 16x16 matrix-core blocks; the waves' partial sums meet in
 // LDS and are added in wave order.  All of a workgroup's bytes are on their way at once, so it takes little more than one way from memory -- as long as
-// there is a workgroup for every CU: MT is 3 where the weights have rows enough (gate and up of 33 x 1024 x 4096: 9.2 us with 3, 14.8 with 1), 1 where not
-// (its w_down: 9.3 with 1, 15.8 with 3), and a small w_down is cut into 8 or 4 rows (16 x 4096 -> 1024: 7.8 us with 4, 10.0 with 16; idle lanes, the matrix core has
-// time).  Two launches for the block where the tiled path takes four (split sums and their joins): 1 x 1024 x 2736 in bf16 10.2 us against 22.7.
+// there is a workgroup for every CU: MT is 3 where the weights have rows enough (gate and up of 33 x 1024 x 4096 in fp16: 8.5 us with 3, 13.6 with 1), 1 where not
+// (its w_down: 9.0 with 1, 14.6 with 3), and a small w_down is cut into 8 or 4 rows (16 x 4096 -> 1024: 8.1 us with 4, 9.8 with 16; idle lanes, the matrix core has
+// time).  Two launches for the block where the tiled path takes four (split sums and their joins): 1 x 1024 x 2736 in bf16 6.1 + 4.5 us against 10.9 + 14.2.
+// What is read more often than once: x, by the workgroups of every slice of the weights, and the weights where MT is 1 and x has more rows.
 template <typename T> __device__ __forceinline__ f32x4 mma16(i32x4 b, i32x4 a, f32x4 c);
 template <> __device__ __forceinline__ f32x4 mma16<__bf16>(i32x4 b, i32x4 a, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);

@@ -10,8 +10,7 @@
 // taken off.  One wave therefore takes a token -- or, with few tokens, a share of a token's heads -- computes the R/2 cosines and sines ONCE
 // (lane p pair p) into a table of its own in LDS, and walks the token's query and key heads with them.  A token has few heads (20 heads of 128
 // channels are three steps of a wave), so what a token begins with is read while the one before it is worked on: its positions, and behind the last heads of
-// the one its first (79 -> 45 us for the norm of 16 + 4 heads of 128 channels at 16382 tokens in bf16, with the sums below as lane permutes and one
-// hardware root a head).
+// the one its first; the sums of a head are lane permutes and its root the hardware's.
 //
 // Layout: a lane holds W pairs = two vectors of W channels.  (i, i + R/2) pairs: vector 0 from the first half, vector 1 from the second;
 // (2i, 2i + 1) pairs: 2W adjacent channels.  No pair spans two lanes, and a lane keeps its pairs from head to head: the weight-gradient sums stay in
@@ -22,8 +21,8 @@
 // W is 16 bytes of a type where pairs, strides and addresses allow it (the gradient in 16-bit types: 8), 8 bytes else, one pair where nothing is aligned.
 //
 // Measured, against the bytes at the 5.1 TB/s of a large copy: rotation of 46800 x 16 x 128 bf16 (383 MB) 80 us, 4.8 TB/s; norm and rotation of 65536 tokens x
-// (4 + 4) x 64 float32 (268 MB) 56 us, 4.8 TB/s; of 16382 x (16 + 4) x 128 bf16 (168 MB) 42 us, 4.0 TB/s, and its gradient (252 MB) 74 us, 3.4 TB/s, + 5 us for
-// the weights' sums.
+// (4 + 4) x 64 float32 (268 MB) 57 us, 4.7 TB/s, and its gradient (403 MB) 87 us, 4.6 TB/s; of 16382 x (16 + 4) x 128 bf16 (168 MB) 43 us, 3.9 TB/s, and its
+// gradient (252 MB) 76 us, 3.3 TB/s, + 5 us for the weights' sums.  The 16-bit gradient has 16 waves a CU (119 registers), each with loads of 8 bytes.
 #include <type_traits>
 
 #include "../common.h"
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(MODE == ROT_NORM_BWD ? ROT_BWD_THREADS : 256) void 
             }
         };
         // Norms in 16-bit types take heads that turn whole apart, by one branch of the wave: with the choice in them too, the gradient of 16 + 4 heads of 128
-        // channels took 82 us instead of 79.  The plain rotation (87 us with the branch, 82 without) and float32 (131 registers, 121) choose pair by pair.
+        // channels took 81 us instead of 79.  The plain rotation (86 us with the branch, 82 without) and float32 (131 registers, 121) choose pair by pair.
         auto turn = [&](float *y, int c) __attribute__((always_inline)) {
             if (NORM && sizeof(T) == 2 && p.R == p.D) turn_pairs(y, c, std::true_type{});
             else turn_pairs(y, c, std::false_type{});
@@ -449,7 +448,7 @@ template <typename T>
 int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStream_t s) {
     constexpr int WV = 16 / sizeof(T);
     const bool bwd = mode == ROT_NORM_BWD;
-    const bool narrow = sizeof(T) == 2 && bwd;  // half the registers, twice the waves: 69 us against 87 for 16 + 4 heads of 128 channels at 16382 tokens
+    const bool narrow = sizeof(T) == 2 && bwd;  // fewer registers: 71 us against 83 for 16 + 4 heads of 128 channels at 16382 tokens
     const int W = !narrow && vec_ok(p, WV, sizeof(T), bwd) ? WV : vec_ok(p, WV / 2, sizeof(T), bwd) ? WV / 2 : 1;
     const int chunks = ((p.D + 1) / 2 + W - 1) / W;
     int lp_log2 = 0;
@@ -472,8 +471,8 @@ int launch_type(RotaryParams &p, RotaryMode mode, void *dw0, void *dw1, hipStrea
     p.items_per_token = (rows + p.rows_per_item - 1) / p.rows_per_item;
     p.items = (unsigned)(tokens * p.items_per_token);  // < 2^31: shares are taken only where tokens are few
     // A step or a few a token are mostly the way from its position to its angles: an item of several tokens then, until it is four steps of the wave (and
-    // its table 256 pairs), as long as there are items enough (6 x 13278 tokens of one 64-channel head in fp16: 16.5 us a
-    // call instead of 36; 13 x 10525 of three of 16 in float32 15 instead of 53)
+    // its table 256 pairs), as long as there are items enough (6 x 13278 tokens of one 64-channel head in fp16: 18 us
+    // instead of 50; 13 x 10525 of three of 16 in float32 16 instead of 69)
     const int P = chunks * W;
     p.group = 1;
     if (shares == 1 && rows <= 4 * row_step) {

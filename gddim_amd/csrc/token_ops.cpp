@@ -90,8 +90,10 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     const bool gated = kind == GEMM_GATE_UP;
     const long long cus = device_cus();
     // Few rows: the weight-streaming kernel, where it is estimated to be faster than tiles.  Its time is what its workgroups read, mostly from L2: their rows of
-    // the weights and their rows of x, once for each workgroup (us of 64 x 1024 x 4096 in fp16 22.3, tiles 30.9; 96 rows 29.6, 32.8; 128 x 256 x 688 bf16 8.5, 18.8;
-    // 1 x 4096 x 14336 70, 85; but 16 x 4096 x 14336 97, 80; 64 rows 217, 91; 96 x 2048 x 8192 78, 46; 96 x 1024 x 4096 float32 61, 55)
+    // the weights and their rows of x, once for each workgroup.  us of gate and up, then of y, in this kernel and (in brackets) in the best tiles, joins with them:
+    // 64 x 1024 x 4096 in fp16 12.9 (14.1), 9.6 (18.6); 96 rows 16.1 (15.6), 12.9 (19.2); 128 x 256 x 688 bf16 5.0 (7.2), 3.6 (10.8); 1 x 4096 x 14336 70 (79), 32 (63);
+    // 64 rows 147 (90), 88 (41); 96 x 2048 x 8192 51 (29), 34 (22); 96 x 1024 x 4096 float32 32 (29), 27 (23).  16 x 4096 x 14336 is where the estimate errs most:
+    // 79 here for gate and up, 97 in the tiles it takes.
     double skinny_us = 1e30;
     int skinny_m = 0, skinny_rows = 16, skinny_tiles = 0;
     long long skinny_grid = 0;
@@ -115,14 +117,15 @@ long long plan_gemm(GemmLaunch &l, int dtype, GemmKind kind) {
     auto stages_of = [&](const GemmProblem &q) { return q.K ? (long long)q.parts * ((q.K + kstage - 1) / kstage) : 1; };
     // Tile and split of the sums by estimated time, in us.  A 256 x 256 tile holds a CU, smaller ones share it by two or more; a CU with c tiles takes c times a
     // stage's time per stage, and a fixed time for the way in and out.  Split sums are written and read again by the join.  The constants are fits to y
-    // = h Wd^T of 16384 x 1024, K = 256 .. 4096, in bf16 (256: 16.5, 23.6, 36.8, 127.9 us; 128: 18.4, 25.6, 40.5, 148.9) and to one and two 128 tiles a CU
-    // (21.6, 24.9 us at K = 1024); operands whose k is not adjacent cost the small tile more (the weights' gradients of 16384 x 1024 x 4096: 432 us with 256,
-    // 554 with 128), and where every CU multiplies, the clock falls: split four ways over all of them these gradients' 192 tiles take 421 us and the join 45.
+    // = h Wd^T of 16384 x 1024, K = 256, 512, 1024, 4096, in bf16 (256: 16.5, 24.0, 40.3, 139.6 us; 128: 18.3, 26.9, 42.5, 163.2) and to one and two 128 tiles a CU
+    // (17, 24 us at K = 1024); operands whose k is not adjacent cost the small tile more (the weights' gradients of 16384 x 1024 x 4096: 392 us with 256,
+    // 488 with 128); split four ways over all CUs these gradients' 192 tiles take 369 us and the join 44.
     // Tiles of 128 x 64 cost more per product but fill narrow matrices and the last round of tiles better.  float32, whose matrix core is 16 times slower: 8192
-    // x 1024 x 4096 gate and up 1.12 ms (1.03 with 128 x 128), 6080 x 192 x 2464 down 71 us (81), dx 120 (150), the weights' gradients 199 (224); gate and up of
-    // 4096 x 256 x 684 37.5 (44).  bf16: 2048 x 1024 x 4096 down 32 us (27), 10069 x 344 x 1208 24 (28), dhidden 49 (54, with 256), of 658 x 184 x 2712 14 (18):
+    // x 1024 x 4096 gate and up 1.11 ms (1.03 with 128 x 128), 6080 x 192 x 2464 down 63 us (92), dx 110 (166), the weights' gradients 174 (200); gate and up of
+    // 4096 x 256 x 684 34.8 (40.9).  bf16: 2048 x 1024 x 4096 down 44 us (37), 10069 x 344 x 1208 25 (28), dhidden 51 (58; 66 with 256), of 658 x 184 x 2712 12 (17):
     // each tile of dhidden waits for the projections it reads, once for every 32 rows of a wave (one, two or four times in a tile).  Through registers a stage takes two to three times as long
-    // (428 x 884 x 2764 in fp16: dhidden 28 us, 43 with 128 x 128; dx 22, 29).
+    // (428 x 884 x 2764 in fp16: dhidden 28 us, 45 with 128 x 128; dx 28, 58).
+    // Where it errs: gate and up that are kept, with few stages (16384 x 64 x 512: 30 us with 256, 18 with 128); profiles/token_ops_tile_times.csv holds these and more.
     struct Cost { double alone, shared; };  // us a stage and tile
     const bool f32 = dtype == GD_F32, dhidden = kind == GEMM_DHIDDEN;
     const Cost wide = f32 ? Cost{2.45, 2.0} : Cost{1.05, kind == GEMM_DW ? 0.6 : dhidden || kind == GEMM_DX ? 0.65 : 0.57};

@@ -70,7 +70,9 @@ class RotaryAxes:
 
     sections[a] channels (even) turn with axis a, in this order; channels behind the last section pass through.  Pair j of a section turns
     by pos * theta^(-2 j / sections[a]); `frequencies` (sum(sections) / 2 radians per unit of position) replaces these.  paired:
-    'interleaved' -- channels (2 p, 2 p + 1) -- or 'halves' -- channels (p, p + sum(sections) / 2).  Keeps one float64 table on `device`."""
+    'interleaved' -- channels (2 p, 2 p + 1) -- or 'halves' -- channels (p, p + sum(sections) / 2).  Keeps one float64 table on `device`, whose memory is
+    like any tensor's: it has to be kept as long as a captured graph that used it is replayed, and until work queued on a stream other than the one it was
+    made on has ended."""
 
     def __init__(self, sections, theta=10000.0, paired="interleaved", device=None, frequencies=None):
         torch = _torch()[0]
@@ -309,7 +311,8 @@ def _workspace(x, fields, backward):
 def gated_ffn(x, w_gate, w_up, w_down, act="silu", save=False):
     """Gated feed-forward block (act(x w_gate^T) * (x w_up^T)) w_down^T: x (..., in), weights as torch.nn.Linear keeps them -- w_gate and w_up
     (hidden, in), w_down (out, hidden) -- act 'silu', 'gelu' or 'gelu_tanh'.  Returns y (..., out); with save=True (y, saved), saved for
-    gated_ffn_backward (the two projections in float32 and their product).  Both projections, the activation and the product are one kernel."""
+    gated_ffn_backward (the two projections in float32 and their product).  Both projections, the activation and the product are one kernel where the
+    sums are not split; where they are (little to fill the chip with), a second one joins them and applies activation and product."""
     x_in = x
     x, w_gate, w_up, w_down, fields = _check_ffn(x, w_gate, w_up, w_down, act)
     rows, F, O = fields[2], fields[4], fields[5]
